@@ -242,16 +242,15 @@ def plain_write(s):
     kept = owner[slots] == token  # of two tokens for one slot the later one stays
 
     def one(x, cache, scale, key):
-        x = x.float()
-        amax = torch.zeros(scale.shape[:2], device=x.device).scatter_reduce(0, block[:, None].expand(-1, x.shape[1]), x.abs().amax(2), "amax")
+        x, b, o = x[kept].float(), block[kept], off[kept]
+        amax = torch.zeros(scale.shape[:2], device=x.device).scatter_reduce(0, b[:, None].expand(-1, x.shape[1]), x.abs().amax(2), "amax")
         old = scale[:, :, 0, 0]
         grown = torch.maximum(old, power_of_two_scale(amax))
         new = torch.where(torch.zeros_like(old).index_fill(0, touched, 1.0) > 0, grown, old)
         ratio = torch.where(old > 0, old / new, torch.ones_like(old))
         # the codes of the touched blocks follow their scale
         cache[touched] = (cache[touched].float() * ratio[touched].view(-1, ratio.shape[1], *([1] * (cache.dim() - 2)))).to(FP8)
-        code = (x / new[block].unsqueeze(2)).clamp(-FP8_MAX, FP8_MAX).to(FP8)[kept]  # [tokens, Hkv, D]
-        b, o = block[kept], off[kept]
+        code = (x / new[b].unsqueeze(2)).clamp(-FP8_MAX, FP8_MAX).to(FP8)  # [tokens, Hkv, D]
         if key:
             cache.permute(0, 3, 1, 2, 4)[b, o] = code.view(*code.shape[:2], -1, 16)
         elif vt:
