@@ -69,8 +69,9 @@ extern "C" {
 enum { PA_DTYPE_BF16 = 0, PA_DTYPE_FP8_E4M3FN = 1 };
 /* quantisation modes, numbered as the reference numbers them
  * (pa_decode_triton_gluon_fp8.py:1753-1790): -1 no scale, 0 one f32 per tensor (read from
- * device memory), 1 one f32 per token and kv-head ([num_blocks, num_kv_heads, block_size, 1]) */
-enum { PA_QUANT_NONE = -1, PA_QUANT_PER_TENSOR = 0, PA_QUANT_PER_TOKEN = 1 };
+ * device memory), 1 one f32 per token and kv-head ([num_blocks, num_kv_heads, block_size, 1]); and, for the
+ * block-granular entry points alone, 2: one f32 per block and kv-head ([num_blocks, num_kv_heads, 1, 1]) */
+enum { PA_QUANT_NONE = -1, PA_QUANT_PER_TENSOR = 0, PA_QUANT_PER_TOKEN = 1, PA_QUANT_PER_BLOCK = 2 };
 
 enum {
   PA_OK = 0,
@@ -302,6 +303,107 @@ int pa_kv_cache_write(const PaKvWriteArgs* args, void* hip_stream);
 int pa_quantize_kv_cache(const void* key_cache_bf16, const void* value_cache_bf16, void* key_cache_fp8,
                          void* value_cache_fp8, float* key_scale, float* value_scale, int64_t num_blocks,
                          int32_t num_kv_heads, int32_t head_size, int32_t block_size, void* hip_stream);
+
+/*
+ * KV-cache write into an FP8 cache that holds ONE scale per block and kv head (args->kv_quant_mode must be
+ * PA_QUANT_PER_BLOCK, key_scale / value_scale [num_blocks, Hkv] at stride_scale_b / stride_scale_h, read and written).
+ * For every block that a live slot of the call lies in, and every kv head:
+ *     s_new = max(s_old, the smallest power of two s with amax <= 448 s),   amax over the finite values of the call's
+ *             rows that stay in the block (2^-126 at least; an all-zero first write leaves 2^-126);
+ *     s_old > 0 and s_new > s_old: every code already in the block becomes e4m3(code * (s_old / s_new)), which for
+ *             scales that are powers of two is a shift of its exponent (exact but for codes that become subnormal);
+ *     a new row becomes e4m3(clamp(x / s_new, -448, 448)), a NaN stays a NaN.
+ * A scale only grows.  A scale of 0 marks an empty block (its codes are not read): whoever hands a block to another
+ * sequence sets its scales to 0, or the new tokens share the old tokens' scale (a coarser one at worst).  Scales must
+ * be finite and >= 0.  Blocks no live slot lies in are left as they are.  Of two tokens with one slot the later one stays; a
+ * slot below 0 or at or beyond num_blocks * block_size is skipped.  One launch, nothing but the caches and the scales
+ * is written, and the result does not depend on the order in which workgroups run.
+ */
+int pa_kv_cache_write_block_scaled(const PaKvWriteArgs* args, int64_t num_blocks, void* hip_stream);
+
+/*
+ * Decode attention at the granularity of cache blocks (one struct for the operators that belong together).  Shapes as
+ * in PaDecodeArgs; N = num_blocks, W = table_width:
+ *   output        bf16 [B, Hkv*Ge, D]          query  bf16 [B, Hkv*Ge, D]
+ *   key_cache     [N, Hkv, D/x, bs, x]         value_cache [N, Hkv, D, bs] or transposed [N, Hkv, bs/x, D, x]
+ *   key_scale, value_scale   by kv_quant_mode: none, one f32, [N, Hkv, bs, 1] or [N, Hkv, 1, 1]
+ *   bounds        bf16 [N, Hkv, 2, D]          row 0 the smallest, row 1 the largest key of a block, per head dim
+ *   selected_blocks  int32 [B, Hkv, K]         logical block numbers (positions in the sequence's row of block_tables)
+ *   selected_counts  int32 [B, Hkv]            how many of them are meant
+ *   lse           f32 [B, Hkv*Ge]              natural logarithm of the row's softmax denominator (with its maximum)
+ *   context_lens  int32 [B], cut at max_context_len and at table_width * block_size; block_tables int32 [B, W]
+ * A block number outside a sequence, or a table entry outside [0, N), contributes nothing and is not followed.
+ */
+typedef struct PaBlockArgs {
+  uint32_t struct_size; /* = sizeof(PaBlockArgs) */
+  int32_t reserved0;    /* 0 */
+
+  void* output;
+  const void* query;
+  const void* key_cache;
+  const void* value_cache;
+  const float* key_scale;
+  const float* value_scale;
+  const int32_t* context_lens;
+  const int32_t* block_tables;
+  const int32_t* q_lens;          /* optional */
+  void* bounds;                   /* written by pa_block_bounds, read by pa_select_blocks */
+  int32_t* selected_blocks;       /* written by pa_select_blocks; optional in pa_block_attention (NULL: every block) */
+  int32_t* selected_counts;       /* written by pa_select_blocks; optional in pa_block_attention (NULL: num_selected) */
+  float* lse;                     /* optional */
+  void* workspace;                /* scratch of workspace_bytes bytes, any contents; 16-byte aligned */
+
+  int32_t num_seqs, num_kv_heads, group_size, q_len, head_size, block_size;
+  int32_t num_blocks, table_width, max_context_len;
+  int32_t kv_dtype, kv_quant_mode, v_transposed;
+  int32_t num_selected;           /* K */
+  int32_t first_blocks, recent_blocks; /* pa_select_blocks: blocks at the two ends that are always selected */
+  int32_t new_tokens;             /* pa_block_bounds: the blocks that hold the last new_tokens tokens; 0: all blocks */
+  float softmax_scale;
+  int32_t reserved1;              /* 0 */
+
+  int64_t stride_out_s, stride_out_h, stride_q_s, stride_q_h;
+  int64_t stride_k_b, stride_k_h, stride_k_c, stride_v_b, stride_v_h, stride_v_2;
+  int64_t stride_kvscale_b, stride_kvscale_h;
+  int64_t stride_bt_s;
+  int64_t stride_bounds_b, stride_bounds_h; /* the [2, D] of a (block, head) is dense */
+  int64_t stride_sel_s, stride_sel_h, stride_cnt_s, stride_lse_s; /* innermost dimensions dense */
+  int64_t workspace_bytes;
+} PaBlockArgs;
+
+uint32_t pa_block_args_size(void);
+
+/*
+ * output[row] = softmax(softmax_scale * q K^T) V over the tokens of the selected blocks (every block without a list)
+ * that the row may see (causal over the sequence's new tokens); rows that see no token, and rows beyond a sequence's
+ * q_lens entry, are written as zero with an lse of -infinity.  Partial results of a cut token axis are held in f32
+ * in the workspace (pa_block_attention_workspace_bytes; 0 when one workgroup takes a sequence's whole axis) and
+ * merged by a second kernel.  P V is accumulated from probabilities carried as two bf16 terms, so the output's one
+ * rounding is the last.  Value rows of all tokens below the context length must be finite: a NaN among a sequence's
+ * new tokens reaches all of the sequence's query rows, as 0 * NaN does.  Cache bytes beyond the context are ignored.
+ */
+int pa_block_attention(const PaBlockArgs* args, void* hip_stream);
+int64_t pa_block_attention_workspace_bytes(const PaBlockArgs* args);
+
+/*
+ * bounds of the blocks of every sequence: the smallest and the largest key (code * scale, in f32) over the block's
+ * tokens below the context length, rounded to bf16; NaN keys are passed over (a head dim without any other value gets
+ * +infinity, -infinity).  With new_tokens > 0 only the blocks that hold the last new_tokens tokens are visited (a
+ * decode step); other blocks' bounds are left as they are.
+ */
+int pa_block_bounds(const PaBlockArgs* args, void* hip_stream);
+
+/*
+ * For every (sequence, kv head) the num_selected blocks with the largest score, as ascending logical block numbers,
+ * -1 behind the last; selected_counts[b, h] of them.  With lo, hi the bounds of a block,
+ *     score = max over the sequence's query rows of the head of   sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d),
+ * an upper bound of q . k over the block's tokens.  Scores are ranked by their value in 64 bits, equal ones by the lower
+ * block number; a row whose sum is not a number is passed over, a block with no other row ranks last.  The first
+ * first_blocks and the last recent_blocks blocks of a sequence are always selected (their sum is at most num_selected).
+ * The workspace takes pa_select_blocks_workspace_bytes.
+ */
+int pa_select_blocks(const PaBlockArgs* args, void* hip_stream);
+int64_t pa_select_blocks_workspace_bytes(const PaBlockArgs* args);
 
 /*
  * Test hook: decodes n FP8 e4m3fn bytes (device pointer) to f32 (device pointer) with the same

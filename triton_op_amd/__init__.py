@@ -8,7 +8,15 @@ from .pa_decode import (  # noqa: F401
     select_partition_size,
 )
 from .kv_cache import kv_cache_write, quantize_kv_cache_symmetric  # noqa: F401
+from .block_attention import (  # noqa: F401
+    BlockAttentionPlan,
+    key_block_bounds,
+    paged_block_attention,
+    plan_block_attention,
+    select_blocks,
+)
 from . import kv_layout, workloads  # noqa: F401
 
 __all__ = ["paged_attention_decode", "plan_decode", "DecodePlan", "select_partition_size", "kv_cache_write",
-           "quantize_kv_cache_symmetric", "kv_layout", "workloads"]
+           "quantize_kv_cache_symmetric", "paged_block_attention", "plan_block_attention", "BlockAttentionPlan",
+           "key_block_bounds", "select_blocks", "kv_layout", "workloads"]

@@ -19,7 +19,7 @@ PA_ERR_SCRATCH_TOO_SMALL = -7
 PA_DECODE_FLAG_REUSE_ITEM_LIST = 1
 PA_DECODE_FLAG_OUTPUT_ONLY = 2
 PA_DTYPE_BF16, PA_DTYPE_FP8_E4M3FN = 0, 1
-PA_QUANT_NONE, PA_QUANT_PER_TENSOR, PA_QUANT_PER_TOKEN = -1, 0, 1
+PA_QUANT_NONE, PA_QUANT_PER_TENSOR, PA_QUANT_PER_TOKEN, PA_QUANT_PER_BLOCK = -1, 0, 1, 2
 
 EXPORTED_SYMBOLS = (
     "pa_decode_abi_version",
@@ -37,6 +37,13 @@ EXPORTED_SYMBOLS = (
     "pa_debug_fp8_decode",
     "pa_kv_cache_write",
     "pa_quantize_kv_cache",
+    "pa_kv_cache_write_block_scaled",
+    "pa_block_args_size",
+    "pa_block_attention",
+    "pa_block_attention_workspace_bytes",
+    "pa_block_bounds",
+    "pa_select_blocks",
+    "pa_select_blocks_workspace_bytes",
 )
 
 
@@ -70,6 +77,25 @@ class PaKvWriteArgs(C.Structure):
         + [(n, C.c_int64) for n in (
             "stride_k_t", "stride_k_h", "stride_v_t", "stride_v_h", "stride_kc_b", "stride_kc_h", "stride_vc_b",
             "stride_vc_h", "stride_scale_b", "stride_scale_h")]
+    )
+
+
+class PaBlockArgs(C.Structure):
+    _fields_ = (
+        [("struct_size", C.c_uint32), ("reserved0", C.c_int32)]
+        + [(n, C.c_void_p) for n in (
+            "output", "query", "key_cache", "value_cache", "key_scale", "value_scale", "context_lens", "block_tables",
+            "q_lens", "bounds", "selected_blocks", "selected_counts", "lse", "workspace")]
+        + [(n, C.c_int32) for n in (
+            "num_seqs", "num_kv_heads", "group_size", "q_len", "head_size", "block_size", "num_blocks", "table_width",
+            "max_context_len", "kv_dtype", "kv_quant_mode", "v_transposed", "num_selected", "first_blocks",
+            "recent_blocks", "new_tokens")]
+        + [("softmax_scale", C.c_float), ("reserved1", C.c_int32)]
+        + [(n, C.c_int64) for n in (
+            "stride_out_s", "stride_out_h", "stride_q_s", "stride_q_h", "stride_k_b", "stride_k_h", "stride_k_c",
+            "stride_v_b", "stride_v_h", "stride_v_2", "stride_kvscale_b", "stride_kvscale_h", "stride_bt_s",
+            "stride_bounds_b", "stride_bounds_h", "stride_sel_s", "stride_sel_h", "stride_cnt_s", "stride_lse_s",
+            "workspace_bytes")]
     )
 
 
@@ -117,12 +143,26 @@ def load_library(path: str = None) -> C.CDLL:
         lib.pa_kv_cache_write.argtypes = [C.POINTER(PaKvWriteArgs), C.c_void_p]
         lib.pa_quantize_kv_cache.restype = C.c_int
         lib.pa_quantize_kv_cache.argtypes = [C.c_void_p] * 6 + [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]
+        lib.pa_kv_cache_write_block_scaled.restype = C.c_int
+        lib.pa_kv_cache_write_block_scaled.argtypes = [C.POINTER(PaKvWriteArgs), C.c_int64, C.c_void_p]
+        lib.pa_block_args_size.restype = C.c_uint32
+        for name in ("pa_block_attention", "pa_block_bounds", "pa_select_blocks"):
+            fn = getattr(lib, name)
+            fn.restype = C.c_int
+            fn.argtypes = [C.POINTER(PaBlockArgs), C.c_void_p]
+        for name in ("pa_block_attention_workspace_bytes", "pa_select_blocks_workspace_bytes"):
+            fn = getattr(lib, name)
+            fn.restype = C.c_int64
+            fn.argtypes = [C.POINTER(PaBlockArgs)]
         if lib.pa_decode_abi_version() != PA_DECODE_ABI_VERSION:
             raise PaDecodeLibraryError("libpa_decode.so has a different ABI version; rebuild it")
         if lib.pa_decode_args_size() != C.sizeof(PaDecodeArgs):
             raise PaDecodeLibraryError(
                 f"PaDecodeArgs is {lib.pa_decode_args_size()} bytes in the library but "
                 f"{C.sizeof(PaDecodeArgs)} in the binding")
+        if lib.pa_block_args_size() != C.sizeof(PaBlockArgs):
+            raise PaDecodeLibraryError(
+                f"PaBlockArgs is {lib.pa_block_args_size()} bytes in the library but {C.sizeof(PaBlockArgs)} in the binding")
         _lib = lib
         return lib
 

@@ -13,11 +13,12 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = [os.path.join(HERE, "csrc", "pa_decode.hip"), os.path.join(HERE, "csrc", "pa_kv_cache.hip")]
+SOURCES = [os.path.join(HERE, "csrc", f) for f in (
+    "pa_decode.hip", "pa_kv_cache.hip", "pa_block_write.hip", "pa_block_attention.hip", "pa_block_select.hip")]
 HEADERS = [os.path.join(HERE, "..", "include", "pa_decode.h")] + [
     os.path.join(HERE, "csrc", h)
     for h in ("pa_common.h", "pa_launch.h", "pa_partition_kernel.h", "pa_partition_shared_kernel.h", "pa_plan_kernel.h",
-              "pa_reduce_kernel.h", "pa_generic_kernel.h")]
+              "pa_reduce_kernel.h", "pa_generic_kernel.h", "pa_block.h")]
 LIB_PATH = os.path.join(HERE, "libpa_decode.so")
 
 HIPCC_FLAGS = [

@@ -64,9 +64,13 @@ def kv_cache_write(
     key_cache: torch.Tensor,     # [blocks, Hkv, D/x, bs, x]  bf16 or float8_e4m3fn
     value_cache: torch.Tensor,   # [blocks, Hkv, D, bs], or transposed [blocks, Hkv, bs/x, D, x]
     slot_mapping: torch.Tensor,  # [num_tokens] int64, block * block_size + offset; negative = skip
-    key_scale: Optional[torch.Tensor] = None,    # FP8 cache: [blocks, Hkv, bs, 1] (written) or 0-dim (read)
-    value_scale: Optional[torch.Tensor] = None,
+    key_scale: Optional[torch.Tensor] = None,    # FP8 cache: [blocks, Hkv, bs, 1] (written), [blocks, Hkv, 1, 1]
+    value_scale: Optional[torch.Tensor] = None,  # (read and written) or 0-dim (read)
 ) -> None:
+    """New tokens into their slots.  With scales [blocks, Hkv, 1, 1] a block's codes share one scale per head: it only
+    grows, by powers of two, and the codes that are already in the block follow it (set a block's scales to 0 when it is
+    handed to another sequence: 0 marks an empty block); of two tokens with one slot the later one stays, and slots
+    outside the cache are skipped."""
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16 or key.shape != value.shape or key.dim() != 3:
         raise ValueError("key and value must be bfloat16 [num_tokens, num_kv_heads, head_size]")
     if not key.is_cuda:
@@ -113,6 +117,11 @@ def kv_cache_write(
             raise ValueError("scales need an FP8 cache")
         if key_scale.dim() == 0:
             mode = _cabi.PA_QUANT_PER_TENSOR
+        elif tuple(key_scale.shape) == (key_cache.shape[0], h, 1, 1) and bs != 1:
+            if key_scale.stride() != value_scale.stride():
+                raise ValueError("key_scale and value_scale must have the same strides")
+            mode = _cabi.PA_QUANT_PER_BLOCK
+            a.stride_scale_b, a.stride_scale_h = key_scale.stride(0), key_scale.stride(1)
         else:
             if tuple(key_scale.shape) != (key_cache.shape[0], h, bs, 1) or key_scale.stride(2) != 1 or \
                     key_scale.stride() != value_scale.stride():
@@ -126,4 +135,11 @@ def kv_cache_write(
     a.stride_kc_b, a.stride_kc_h = key_cache.stride(0), key_cache.stride(1)
     a.stride_vc_b, a.stride_vc_h = value_cache.stride(0), value_cache.stride(1)
     lib = _cabi.load_library()
+    if mode == _cabi.PA_QUANT_PER_BLOCK:
+        if key_cache.shape[0] != value_cache.shape[0]:
+            raise ValueError(f"key_cache has {key_cache.shape[0]} blocks, value_cache {value_cache.shape[0]}")
+        with torch.cuda.device(key.device):
+            _cabi.check(lib.pa_kv_cache_write_block_scaled(C.byref(a), key_cache.shape[0], _stream(key.device)),
+                        "pa_kv_cache_write_block_scaled")
+        return
     _cabi.check(lib.pa_kv_cache_write(C.byref(a), _stream(key.device)), "pa_kv_cache_write")
