@@ -15,96 +15,377 @@ __device__ __forceinline__ int block_context(const PaBlockArgs& a, int b, int ax
 }
 
 // ---- bounds -----------------------------------------------------------------------------------------------------------
-// One wave per (sequence, visited block, kv head); lane l owns head dims l, l + 64, ...
-template <int D, bool FP8>
-__global__ __launch_bounds__(64) void pa_block_bounds_kernel(const PaBlockArgs a, const int axis, const int visits) {
-  const int lane = threadIdx.x;
-  const int h = (int)(blockIdx.x % (unsigned)a.num_kv_heads);
-  const int item = (int)(blockIdx.x / (unsigned)a.num_kv_heads);
-  const int b = item / visits;
-  const int ctx = block_context(a, b, axis);
+//   lo_d = min_t k_td scale_t, hi_d = max_t k_td scale_t     over the block's tokens below the context length
+//
+// Read-bound: head size bytes per token and 4 D written per block.  LPC lanes share a 16-byte chunk row of the block and
+// take its tokens in turn (behind the last live token they take it again, which changes no extremum); every lane keeps
+// [-lo, hi] of its chunk's head dims, so that all is maxima, and the lanes of a chunk row then halve what they hold with every
+// exchange (a lane sends the half its partner keeps): 15 exchanges instead of 16 for each of log2(LPC) steps.
+// FP8 codes are exact in 16-bit floats, where two maxima are one instruction (and a maximum passes over NaN); per-token
+// scales need 32 bits.
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+enum { kBoundsFp8 = 0, kBoundsFp8Token = 1, kBoundsBf16 = 2 };
+
+__device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t word, bool high_half) {
+  union {
+    f16x2 v;
+    uint32_t u;
+  } r;
+  r.v = high_half ? __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, true))
+                  : __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, false));
+  return r.u;
+}
+
+template <int KIND>
+struct BoundSlot;
+// two head dims as 16-bit floats
+template <>
+struct BoundSlot<kBoundsFp8> {
+  static constexpr int kDims = 2;
+  uint32_t u = 0xfc00fc00u;  // -infinity
+  __device__ __forceinline__ void take(uint32_t o) {
+    const f16x2 x = __builtin_bit_cast(f16x2, u), y = __builtin_bit_cast(f16x2, o);
+    u = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+  }
+  __device__ __forceinline__ uint32_t bits() const { return u; }
+  __device__ __forceinline__ float dim(int i) const { return (float)__builtin_bit_cast(f16x2, u)[i]; }
+};
+// one head dim in 32 bits
+struct BoundSlot32 {
+  static constexpr int kDims = 1;
+  float x = -INFINITY;
+  __device__ __forceinline__ void take(uint32_t o) { x = fmaxf(x, __uint_as_float(o)); }
+  __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(x); }
+  __device__ __forceinline__ float dim(int) const { return x; }
+};
+template <>
+struct BoundSlot<kBoundsFp8Token> : BoundSlot32 {};
+template <>
+struct BoundSlot<kBoundsBf16> : BoundSlot32 {};
+
+// SPLIT: the four waves of a workgroup share one (sequence, block, kv head) and meet in LDS (blocks of 64 tokens and more);
+// otherwise each has its own.
+template <int D, int KIND, bool SPLIT>
+__global__ __launch_bounds__(256) void pa_block_bounds_kernel(const PaBlockArgs a, const int axis, const int visits, const unsigned items) {
+  typedef BoundSlot<KIND> Slot;
+  constexpr bool FP8 = KIND != kBoundsBf16;
+  constexpr int X = FP8 ? 16 : 8;
+  constexpr int LPC = 64 / (D / X);         // lanes of a chunk row
+  constexpr int HALF = X / Slot::kDims;     // slots of -lo, and as many of hi
+  constexpr int KEEP = 2 * HALF / LPC;      // slots a lane is left with
+  constexpr int U = 16 / LPC < 4 ? 16 / LPC : 4;  // loads in flight (a 16-token block has 16 / LPC for a lane)
+  static_assert(KEEP >= 1, "a lane is left with something");
+  __shared__ uint32_t meet[SPLIT ? 3 : 1][SPLIT ? KEEP : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned item = SPLIT ? blockIdx.x : blockIdx.x * 4 + wave;
+  if (item >= items) return;
+  const int h = (int)(item % (unsigned)a.num_kv_heads);
+  const unsigned visit = item / (unsigned)a.num_kv_heads;
+  const int b = (int)(visit / (unsigned)visits);
   const int bs = a.block_size;
+  int ctx = sload_i32(a.context_lens + b);
+  ctx = ctx > axis ? axis : ctx;
   const int first = a.new_tokens > 0 ? (ctx > a.new_tokens ? ctx - a.new_tokens : 0) / bs : 0;
-  const int at = first + item % visits;
-  if (at * bs >= ctx) return;
-  const int page = a.block_tables[(int64_t)b * a.stride_bt_s + at];
+  const int at = first + (int)(visit % (unsigned)visits);
+  if (at >= (ctx + bs - 1) / bs) return;
+  const int page = sload_i32(a.block_tables + (int64_t)b * a.stride_bt_s + at);
   if ((unsigned)page >= (unsigned)a.num_blocks) return;
   const int live = ctx - at * bs < bs ? ctx - at * bs : bs;
-  constexpr int X = FP8 ? 16 : 8;
-  const char* kp = (const char*)a.key_cache + ((int64_t)page * a.stride_k_b + (int64_t)h * a.stride_k_h) * (FP8 ? 1 : 2);
-  const float* sp = a.key_scale + (int64_t)page * a.stride_kvscale_b + (int64_t)h * a.stride_kvscale_h;
-  __bf16* out = (__bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)h * a.stride_bounds_h;
-  for (int d = lane; d < D; d += 64) {
-    float lo = INFINITY, hi = -INFINITY;
-    for (int t = 0; t < live; ++t) {
-      const int64_t e = (int64_t)(d / X) * a.stride_k_c + t * X + d % X;
-      float x;
-      if constexpr (FP8)
-        x = __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)kp)[e], 0);
-      else
-        x = bf16_bits_to_f32(((const uint16_t*)kp)[e]);
-      if (a.kv_quant_mode == PA_QUANT_PER_TENSOR) x *= a.key_scale[0];
-      if (a.kv_quant_mode == PA_QUANT_PER_TOKEN) x *= sp[t];
-      if (a.kv_quant_mode == PA_QUANT_PER_BLOCK) x *= sp[0];
-      if (x < lo) lo = x;
-      if (x > hi) hi = x;
+  const char* kp = (const char*)a.key_cache + ((int64_t)page * a.stride_k_b + (int64_t)h * a.stride_k_h + (int64_t)(lane / LPC) * a.stride_k_c) * (FP8 ? 1 : 2);
+  const int64_t so = (int64_t)page * a.stride_kvscale_b + (int64_t)h * a.stride_kvscale_h;
+  float scale = 1.f;
+  if (a.kv_quant_mode == PA_QUANT_PER_TENSOR) scale = sload_f32(a.key_scale);
+  if (a.kv_quant_mode == PA_QUANT_PER_BLOCK) scale = sload_f32(a.key_scale + so);
+
+  Slot slot[2 * HALF];  // [-lo, hi]
+  constexpr int kTurn = LPC * U * (SPLIT ? 4 : 1);
+  for (int t0 = (SPLIT ? wave * LPC * U : 0) + lane % LPC; t0 - lane % LPC < live; t0 += kTurn) {
+    u32x4 w[U];
+    float ts[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * LPC < live ? t0 + u * LPC : live - 1;
+      w[u] = load16_stream(kp + t * 16);
+      if constexpr (KIND == kBoundsFp8Token) ts[u] = a.key_scale[so + t];
     }
-    out[d] = (__bf16)lo;
-    out[D + d] = (__bf16)hi;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (KIND == kBoundsFp8) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t p = fp8x2_to_f16x2(w[u][i], e);
+            slot[2 * i + e].take(p ^ 0x80008000u);
+            slot[HALF + 2 * i + e].take(p);
+          }
+        } else if constexpr (KIND == kBoundsFp8Token) {
+          const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 0) * ts[u], __builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 1) * ts[u],
+                              __builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 2) * ts[u], __builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 3) * ts[u]};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            slot[4 * i + e].take(__float_as_uint(-x[e]));
+            slot[HALF + 4 * i + e].take(__float_as_uint(x[e]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x = e ? w[u][i] & 0xffff0000u : w[u][i] << 16;
+            slot[2 * i + e].take(x ^ 0x80000000u);
+            slot[HALF + 2 * i + e].take(x);
+          }
+        }
+      }
+    }
+  }
+  // ---- the lanes of a chunk row: step k pairs lanes 2^k apart, the lane with bit k set keeps the upper half --------------------
+#pragma unroll
+  for (int k = 0, n = HALF; (1 << k) < LPC; ++k, n /= 2) {
+    const bool upper = (lane >> k) & 1;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const uint32_t keep = upper ? slot[n + i].bits() : slot[i].bits(), send = upper ? slot[i].bits() : slot[n + i].bits();
+      Slot s;
+      s.take(keep);
+      s.take((uint32_t)__shfl_xor((int)send, 1 << k));
+      slot[i] = s;
+    }
+  }
+  if constexpr (SPLIT) {
+    if (wave > 0) {
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i) meet[wave - 1][i][lane] = slot[i].bits();
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+#pragma unroll
+      for (int o = 0; o < 3; ++o) slot[i].take(meet[o][i][lane]);
+    }
+  }
+  // the slots the lane is left with: KEEP of them from `base` on, all of one bound
+  int base = 0;
+#pragma unroll
+  for (int k = 0; (1 << k) < LPC; ++k) base += ((lane >> k) & 1) * (HALF >> k);
+  const bool is_hi = base >= HALF;
+  const float sign = is_hi ? scale : -scale;
+  // (a negative scale turns the smallest code into the largest key)
+  __bf16* out = (__bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)h * a.stride_bounds_h + (is_hi != (scale < 0.f) ? D : 0) +
+                lane / LPC * X + (is_hi ? base - HALF : base) * Slot::kDims;
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) {
+#pragma unroll
+    for (int e = 0; e < Slot::kDims; ++e) out[i * Slot::kDims + e] = (__bf16)(slot[i].dim(e) * sign);
   }
 }
 
+template <int D, int KIND>
+int launch_bounds(const PaBlockArgs& a, int axis, int visits, hipStream_t s) {
+  const int64_t items = (int64_t)a.num_seqs * visits * a.num_kv_heads;
+  if (items > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
+  if (a.block_size > 16) return pa_launch(pa_block_bounds_kernel<D, KIND, true>, dim3((unsigned)items), dim3(256), 0, s, a, axis, visits, (unsigned)items);
+  return pa_launch(pa_block_bounds_kernel<D, KIND, false>, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, a, axis, visits, (unsigned)items);
+}
+
+template <int D>
+int launch_bounds(const PaBlockArgs& a, int axis, int visits, hipStream_t s) {
+  if (a.kv_dtype == PA_DTYPE_BF16) return launch_bounds<D, kBoundsBf16>(a, axis, visits, s);
+  if (a.kv_quant_mode == PA_QUANT_PER_TOKEN) return launch_bounds<D, kBoundsFp8Token>(a, axis, visits, s);
+  return launch_bounds<D, kBoundsFp8>(a, axis, visits, s);
+}
+
 // ---- scores ------------------------------------------------------------------------------------------------------------
-// a score as a key whose unsigned order is the scores' order; forced blocks have the largest key, which no score has
-constexpr unsigned long long kForcedKey = ~0ull;
+//   score(block) = max over rows r of x_r,   x_r = sum_d q+_rd hi_d + q-_rd lo_d      (q+ = max(q, 0), q- = min(q, 0))
+//
+// The ranking is by the scores' values in 64 bits, but almost every block is decided by less.  pa_block_score_kernel forms
+// s_r = x_r in 32 bits on v_mfma_f32_16x16x32_bf16 (blocks are the rows, query rows the columns, [lo, hi] against [q-, q+] the
+// 2 D reduction indices) and, with the sign bits cleared, a_r = sum of the terms' magnitudes.  The terms are exact in 32 bits;
+// a sum of 2 D of them in any order, rounded or cut at every step, is off by at most 2 D 2^-23 a_r, so the score lies
+// within e = max_r (2 D 2^-23 a_r) of s = max_r s_r.  The workspace holds (s, e) of every block; e = infinity says that the
+// 32-bit sums decide nothing (an infinity or NaN among them, or a table entry outside the cache).
+// Read-bound: 4 D bytes per block and head against 2 * 2 D / 32 MFMAs per 16 of them.
+struct BlockScore {
+  float s, e;
+};
+
+// lane exchanges inside a row of 16 lanes (DPP): the maximum over the row
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float row16_max(float v) {
+  return dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));  // quad_perm swaps, half mirror, mirror
+}
+
+constexpr int kScoreWaves = 4;
+
+// [lo, hi] against [q-, q+] of one 16-row tile as MFMA operands: operand c of lane l at (c * 64 + l) * 16 bytes
+template <int D>
+__device__ __forceinline__ void stage_query(const PaBlockArgs& a, int b, int h, int rows_valid, int tiles, u32x4* q_lds, int tid, int threads) {
+  constexpr int KM = D / 32;
+  const int Ge = a.q_len * a.group_size;
+  for (int i = tid; i < tiles * KM * 64; i += threads) {
+    const int l = i & 63, c = (i >> 6) % KM, tile = i / (64 * KM);
+    const int row = 16 * tile + (l & 15);
+    u32x4 q = {0, 0, 0, 0};
+    if (row < rows_valid)
+      q = load16((const __bf16*)a.query + (int64_t)b * a.stride_q_s + (int64_t)(h * Ge + row) * a.stride_q_h + 32 * c + 8 * (l >> 4));
+    u32x4 neg, pos;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      // (a NaN goes to both sides; -0 is 0 on either)
+      const uint32_t lo = q[w] & 0xffffu, hi = q[w] >> 16;
+      const uint32_t lo_neg = lo >> 15, hi_neg = hi >> 15, lo_nan = (lo & 0x7fffu) > 0x7f80u, hi_nan = (hi & 0x7fffu) > 0x7f80u;
+      neg[w] = (lo_neg | lo_nan ? lo : 0u) | (hi_neg | hi_nan ? hi << 16 : 0u);
+      pos[w] = (!lo_neg | lo_nan ? lo : 0u) | (!hi_neg | hi_nan ? hi << 16 : 0u);
+    }
+    q_lds[(tile * 2 * KM + c) * 64 + l] = neg;
+    q_lds[(tile * 2 * KM + KM + c) * 64 + l] = pos;
+  }
+}
+
+// One wave scores 16 blocks (blocks at .. at + 15 of the sequence, those below `end`) and writes them at out[at ..].
+template <int D>
+struct ScoreTile {
+  static constexpr int KM = D / 32;
+  u32x4 box[2 * KM];
+  bool ok;
+  __device__ __forceinline__ void load(const PaBlockArgs& a, const int* table, int h, int at, int end, int lane) {
+    const int i = at + (lane & 15);
+    const int page = i < end ? table[i] : 0;
+    ok = (unsigned)page < (unsigned)a.num_blocks;
+    const __bf16* p = (const __bf16*)a.bounds + (int64_t)(ok ? page : 0) * a.stride_bounds_b + (int64_t)h * a.stride_bounds_h + 8 * (lane >> 4);
+#pragma unroll
+    for (int c = 0; c < 2 * KM; ++c) box[c] = load16_stream(p + 32 * c);
+  }
+  __device__ __forceinline__ void score(const u32x4* q_lds, int tiles, int rows_valid, BlockScore* out, int at, int end, int lane) const {
+    constexpr float kBound = 2 * D * 0x1p-23f;
+    const int li = lane & 15, kg = lane >> 4;
+    f32x4 best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, off = {0.f, 0.f, 0.f, 0.f};
+    for (int tile = 0; tile < tiles; ++tile) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f}, m = s;
+#pragma unroll
+      for (int c = 0; c < 2 * KM; ++c) {
+        Bf16x8Bits x, q, xa, qa;
+        x.u = box[c];
+        q.u = q_lds[(tile * 2 * KM + c) * 64 + lane];
+        xa.u = x.u & 0x7fff7fffu;
+        qa.u = q.u & 0x7fff7fffu;
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, q.v, s, 0, 0, 0);
+        m = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa.v, qa.v, m, 0, 0, 0);
+      }
+      if (16 * tile + li < rows_valid) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          best[r] = fmaxf(best[r], s[r]);
+          // (infinite or NaN magnitudes: no bound)
+          off[r] = m[r] < 0x1p126f ? fmaxf(off[r], m[r] * kBound + 0x1p-100f) : INFINITY;
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      best[r] = row16_max(best[r]);
+      off[r] = row16_max(off[r]);
+    }
+    // lane group kg holds blocks 4 kg .. 4 kg + 3; lane li < 4 of it writes block 4 kg + li (the entry that lane loaded: 4 kg + li)
+    const bool entry_ok = __shfl((int)ok, 4 * kg + (li & 3));
+    const int i = at + 4 * kg + li;
+    if (li < 4 && i < end) {
+      BlockScore v;
+      v.s = li == 0 ? best[0] : li == 1 ? best[1] : li == 2 ? best[2] : best[3];
+      v.e = li == 0 ? off[0] : li == 1 ? off[1] : li == 2 ? off[2] : off[3];
+      if (!entry_ok || !(v.s > -INFINITY)) v.e = INFINITY;
+      out[i] = v;
+    }
+  }
+};
+
+// grid: (stretches of `chunk` blocks, a multiple of 64) x (sequence, kv head)
+template <int D>
+__global__ __launch_bounds__(64 * kScoreWaves) void pa_block_score_kernel(const PaBlockArgs a, const int axis, const int axis_blocks, const int chunk) {
+  extern __shared__ __attribute__((aligned(16))) u32x4 q_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = (axis_blocks + chunk - 1) / chunk;
+  const unsigned bh = blockIdx.x / (unsigned)chunks;
+  const int h = (int)(bh % (unsigned)a.num_kv_heads), b = (int)(bh / (unsigned)a.num_kv_heads);
+  const int nb = (block_context(a, b, axis) + a.block_size - 1) / a.block_size;
+  const int begin = (int)(blockIdx.x % (unsigned)chunks) * chunk;
+  const int end = min(begin + chunk, nb - a.recent_blocks);
+  if (nb <= a.num_selected || begin >= end) return;  // (every block is taken, or these blocks are: nobody reads their scores)
+  int qb = a.q_lens ? a.q_lens[b] : a.q_len;
+  qb = qb < 0 ? 0 : (qb > a.q_len ? a.q_len : qb);
+  const int rows_valid = qb * a.group_size, tiles = (rows_valid + 15) / 16;
+  const int* table = a.block_tables + (int64_t)b * a.stride_bt_s;
+  BlockScore* out = (BlockScore*)a.workspace + (int64_t)bh * axis_blocks;
+  ScoreTile<D> t;
+  int at = begin + 16 * wave;
+  if (at < end) t.load(a, table, h, at, end, lane);
+  stage_query<D>(a, b, h, rows_valid, tiles, q_lds, threadIdx.x, 64 * kScoreWaves);
+  __syncthreads();
+  for (; at < end; at += 16 * kScoreWaves) {
+    const ScoreTile<D> now = t;
+    if (at + 16 * kScoreWaves < end) t.load(a, table, h, at + 16 * kScoreWaves, end, lane);
+    now.score(q_lds, tiles, rows_valid, out, at, end, lane);
+  }
+}
+
+// a score as a key whose unsigned order is the scores' order
 __device__ __forceinline__ unsigned long long score_key(double s) {
-  if (s != s) s = -INFINITY;  // no row had a number
-  s = s + 0.0;                // -0 and +0 are equal scores
+  s = s + 0.0;  // -0 and +0 are equal scores
   const unsigned long long u = (unsigned long long)__double_as_longlong(s);
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-// One wave per (sequence, kv head, block): the key of every block into the workspace [B, Hkv, axis blocks].
-template <int D>
-__global__ __launch_bounds__(64) void pa_block_score_kernel(const PaBlockArgs a, const int axis, const int axis_blocks) {
-  const int lane = threadIdx.x;
-  const int h = (int)(blockIdx.x % (unsigned)a.num_kv_heads);
-  const unsigned item = blockIdx.x / (unsigned)a.num_kv_heads;
-  const int b = (int)(item / (unsigned)axis_blocks), at = (int)(item % (unsigned)axis_blocks);
-  const int ctx = block_context(a, b, axis);
-  const int nb = (ctx + a.block_size - 1) / a.block_size;
-  if (at >= nb) return;
-  unsigned long long* key = (unsigned long long*)a.workspace + ((int64_t)b * a.num_kv_heads + h) * axis_blocks + at;
-  if (at < a.first_blocks || at >= nb - a.recent_blocks) {
-    if (lane == 0) *key = kForcedKey;
-    return;
-  }
-  const int page = a.block_tables[(int64_t)b * a.stride_bt_s + at];
+// The key of one block's score in 64 bits, by one wave: 8 rows at a time, 8 lanes to a row, 8 head dims of D to a lane and
+// turn.  Products of bf16 numbers are exact in 64 bits, and so are their sums unless the terms are 2^37 apart.
+__device__ __forceinline__ unsigned long long exact_key(const PaBlockArgs& a, int b, int h, int page, int rows_valid, int lane) {
   double best = -INFINITY;
   if ((unsigned)page < (unsigned)a.num_blocks) {
+    const int D = a.head_size, Ge = a.q_len * a.group_size;
     const __bf16* box = (const __bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)h * a.stride_bounds_h;
-    int qb = a.q_lens ? a.q_lens[b] : a.q_len;
-    qb = qb > a.q_len ? a.q_len : qb;
-    const int Ge = a.q_len * a.group_size;
-    for (int row = 0; row < qb * a.group_size; ++row) {
-      const __bf16* q = (const __bf16*)a.query + (int64_t)b * a.stride_q_s + (int64_t)(h * Ge + row) * a.stride_q_h;
+    for (int row0 = 0; row0 < rows_valid; row0 += 8) {
+      const int row = row0 + (lane >> 3);
+      const __bf16* q = (const __bf16*)a.query + (int64_t)b * a.stride_q_s + (int64_t)(h * Ge + (row < rows_valid ? row : row0)) * a.stride_q_h;
       double s = 0.0;
-      for (int d = lane; d < D; d += 64) {
-        const double x = (double)(float)q[d];
-        s += (x > 0.0 ? x : 0.0) * (double)(float)box[D + d] + (x < 0.0 ? x : 0.0) * (double)(float)box[d];
+      for (int d = 8 * (lane & 7); d < D; d += 64) {
+        const u32x4 x = load16(q + d), lo = load16(box + d), hi = load16(box + D + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int sh = 16 * (e & 1);
+          const float qe = bf16_bits_to_f32((x[e >> 1] >> sh) & 0xffffu);
+          const double l = (double)bf16_bits_to_f32((lo[e >> 1] >> sh) & 0xffffu), u = (double)bf16_bits_to_f32((hi[e >> 1] >> sh) & 0xffffu);
+          s += (double)(qe < 0.f ? 0.f : qe) * u + (double)(qe > 0.f ? 0.f : qe) * l;  // (0 * infinity is NaN in either)
+        }
       }
-      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-      if (s == INFINITY) s = 0x1.fffffffffffffp1023;
-      if (s > best) best = s;  // (a NaN is passed over)
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor(s, o);
+      if (s == INFINITY) s = 0x1.fffffffffffffp1023;  // (below the blocks that are always taken)
+      if (row < rows_valid && s > best) best = s;     // (a NaN is passed over)
+    }
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) {
+      const double t = __shfl_xor(best, o);
+      if (t > best) best = t;
     }
   }
-  if (lane == 0) *key = score_key(best);
+  return score_key(best);
 }
 
 // ---- selection -----------------------------------------------------------------------------------------------------------
-// One workgroup per (sequence, kv head): the K-th largest key by eight passes over its bytes, then the blocks above it
-// and the first of the blocks that equal it, in ascending order.
-constexpr int kSelectThreads = 1024;
+// One workgroup per (sequence, kv head).  The blocks are counted into kBins equal intervals of s; the one in which the count
+// from above reaches `want` holds the threshold, up to the errors e.  Blocks that are above it by more than the
+// errors are taken, blocks below it by more are not, and the few between (the candidates) are ranked by their scores in
+// 64 bits.  With a score that 32 bits do not bound, or more candidates than the list holds (many equal blocks), every score is
+// formed in 64 bits and the threshold is found by eight passes over the keys' bytes.
+// Bound by latency, not by bytes (8 per block, from L2).
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kBins = 2048;
+constexpr int kCandidates = 512;
+constexpr int kFlagWords = 2048;  // 32 blocks each
+
 // exclusive prefix sum of x over the workgroup and its total
 __device__ __forceinline__ int workgroup_scan(int x, int* wave_sums, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -119,7 +400,8 @@ __device__ __forceinline__ int workgroup_scan(int x, int* wave_sums, int& total)
   __syncthreads();
   int before = 0;
   total = 0;
-  for (int w = 0; w < kSelectThreads / 64; ++w) {
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
     const int v = wave_sums[w];
     before += w < wave ? v : 0;
     total += v;
@@ -128,13 +410,16 @@ __device__ __forceinline__ int workgroup_scan(int x, int* wave_sums, int& total)
 }
 
 __global__ __launch_bounds__(kSelectThreads) void pa_block_select_kernel(const PaBlockArgs a, const int axis, const int axis_blocks) {
-  __shared__ int hist[256];
-  __shared__ int wave_sums[kSelectThreads / 64];
-  __shared__ int digit, above;
-  const int tid = threadIdx.x;
+  __shared__ int hist[kBins];
+  __shared__ uint32_t flags[kFlagWords];
+  __shared__ unsigned long long cand_key[kCandidates];
+  __shared__ int cand[kCandidates];
+  __shared__ int wave_sums[kSelectWaves];
+  __shared__ float red[4][kSelectWaves];
+  __shared__ int found[2], num_cand, num_in;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = (int)(blockIdx.x % (unsigned)a.num_kv_heads), b = (int)(blockIdx.x / (unsigned)a.num_kv_heads);
-  const int ctx = block_context(a, b, axis);
-  const int nb = (ctx + a.block_size - 1) / a.block_size;
+  const int nb = (block_context(a, b, axis) + a.block_size - 1) / a.block_size;
   const int K = a.num_selected;
   int32_t* out = a.selected_blocks + (int64_t)b * a.stride_sel_s + (int64_t)h * a.stride_sel_h;
   const int count = nb < K ? nb : K;
@@ -144,40 +429,175 @@ __global__ __launch_bounds__(kSelectThreads) void pa_block_select_kernel(const P
     for (int i = tid; i < nb; i += kSelectThreads) out[i] = i;
     return;
   }
-  const unsigned long long* key = (const unsigned long long*)a.workspace + ((int64_t)b * a.num_kv_heads + h) * axis_blocks;
+  // blocks [begin, end) have scores; `want` of them are taken (nb > K >= first + recent: the two ends do not meet)
+  const int begin = a.first_blocks, end = nb - a.recent_blocks;
+  const int want = K - a.first_blocks - a.recent_blocks;
+  int qb = a.q_lens ? a.q_lens[b] : a.q_len;
+  qb = qb < 0 ? 0 : (qb > a.q_len ? a.q_len : qb);
+  const int rows_valid = qb * a.group_size;
+  const int* table = a.block_tables + (int64_t)b * a.stride_bt_s;
+  const BlockScore* score = (const BlockScore*)a.workspace + (int64_t)blockIdx.x * axis_blocks;
+
+  bool by_32 = nb <= 32 * kFlagWords;
+  if (by_32 && want > 0) {
+    // ---- range of s, largest e ----------------------------------------------------------------------------------------
+    float mn = INFINITY, mx = -INFINITY, E = 0.f;
+    for (int i = begin + tid; i < end; i += kSelectThreads) {
+      const BlockScore v = score[i];
+      mn = fminf(mn, v.s);
+      mx = fmaxf(mx, v.s);
+      E = fmaxf(E, v.e);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      mn = fminf(mn, __shfl_xor(mn, o));
+      mx = fmaxf(mx, __shfl_xor(mx, o));
+      E = fmaxf(E, __shfl_xor(E, o));
+    }
+    if (lane == 0) {
+      red[0][wave] = mn;
+      red[1][wave] = mx;
+      red[2][wave] = E;
+    }
+    for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
+    if (tid == 0) num_cand = num_in = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; ++w) {
+      mn = fminf(mn, red[0][w]);
+      mx = fmaxf(mx, red[1][w]);
+      E = fmaxf(E, red[2][w]);
+    }
+    by_32 = E < INFINITY;
+    if (by_32) {
+      // a monotone map of the scores to bins (a range that overflows puts everything into bin 0)
+      const float scale = mx - mn > 0.f ? (float)(kBins - 1) / (mx - mn) : 0.f;
+      auto bin = [&](float s) {
+        const float x = (s - mn) * scale;
+        return x >= (float)(kBins - 1) ? kBins - 1 : (x > 0.f ? (int)x : 0);
+      };
+      for (int i = begin + tid; i < end; i += kSelectThreads) atomicAdd(&hist[bin(score[i].s)], 1);
+      __syncthreads();
+      // the bin in which the count from above reaches `want`: a thread owns four bins, the highest first
+      constexpr int kOwn = kBins / kSelectThreads;
+      int own[kOwn], sum = 0, total;
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) sum += own[k] = hist[kBins - 1 - (kOwn * tid + k)];
+      int before = workgroup_scan(sum, wave_sums, total);
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) {
+        if (before < want && before + own[k] >= want) found[0] = kBins - 1 - (kOwn * tid + k);
+        before += own[k];
+      }
+      __syncthreads();
+      const int edge = found[0];
+      // ---- taken, candidate or neither: a wave looks at 64 consecutive blocks ----------------------------------------------
+      for (int i0 = 64 * wave; i0 < nb; i0 += 64 * kSelectWaves) {
+        const int i = i0 + lane;
+        bool in = i < nb && (i < begin || i >= end), maybe = false;
+        if (i >= begin && i < end) {
+          const BlockScore v = score[i];
+          // (s +- (e + E), with room for the roundings here: e is at least 2^-16 of |s|)
+          const float slack = (v.e + E) * 1.01f;
+          in = bin(v.s - slack) > edge;
+          maybe = !in && bin(v.s + slack) >= edge;
+          if (in) atomicAdd(&num_in, 1);
+        }
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+        if (lane < 2) flags[(i0 >> 5) + lane] = (uint32_t)(mask >> (32 * lane));
+        if (maybe) {
+          const int at = atomicAdd(&num_cand, 1);
+          if (at < kCandidates) cand[at] = i;
+        }
+      }
+      __syncthreads();
+      by_32 = num_cand <= kCandidates;
+    }
+    if (by_32) {
+      const int n = num_cand, take = want - num_in;
+      if (take < n) {
+        for (int c = wave; c < n; c += kSelectWaves) {
+          const unsigned long long k = exact_key(a, b, h, table[cand[c]], rows_valid, lane);
+          if (lane == 0) cand_key[c] = k;
+        }
+      }
+      __syncthreads();
+      for (int c = tid; c < n; c += kSelectThreads) {
+        const unsigned long long k = cand_key[c];
+        const int at = cand[c];
+        int rank = 0;
+        if (take < n)
+          for (int o = 0; o < n; ++o) rank += cand_key[o] > k || (cand_key[o] == k && cand[o] < at);
+        if (rank < take) atomicOr(&flags[at >> 5], 1u << (at & 31));
+      }
+      __syncthreads();
+    }
+  } else if (by_32) {
+    for (int i0 = 64 * wave; i0 < nb; i0 += 64 * kSelectWaves) {
+      const int i = i0 + lane;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(i < nb && (i < begin || i >= end));
+      if (lane < 2) flags[(i0 >> 5) + lane] = (uint32_t)(mask >> (32 * lane));
+    }
+    __syncthreads();
+  }
+  if (by_32) {
+    // the flags' blocks in ascending order
+    const int words = (nb + 31) >> 5;
+    int done = 0;
+    for (int w0 = 0; w0 < words; w0 += kSelectThreads) {
+      uint32_t f = w0 + tid < words ? flags[w0 + tid] : 0;
+      int total;
+      int at = done + workgroup_scan(__builtin_popcount(f), wave_sums, total);
+      done += total;
+      while (f) {
+        out[at++] = 32 * (w0 + tid) + __builtin_ctz(f);
+        f &= f - 1;
+      }
+    }
+    return;
+  }
+
+  // ---- every score in 64 bits ----------------------------------------------------------------------------------------------
+  unsigned long long* key = (unsigned long long*)a.workspace + (int64_t)blockIdx.x * axis_blocks;
+  __syncthreads();  // everybody is done with the 32-bit scores
+  for (int i = begin + wave; i < end; i += kSelectWaves) {
+    const unsigned long long k = exact_key(a, b, h, table[i], rows_valid, lane);
+    if (lane == 0) key[i] = k;
+  }
+  __threadfence_block();
+  __syncthreads();
   unsigned long long prefix = 0;
-  int want = K;  // of the keys that share the digits fixed so far, how many are still to be taken
-  for (int shift = 56; shift >= 0; shift -= 8) {
+  int left = want;  // of the keys that share the digits fixed so far, how many are still to be taken
+  for (int shift = 56; shift >= 0 && want > 0; shift -= 8) {
     for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < nb; i += kSelectThreads) {
+    for (int i = begin + tid; i < end; i += kSelectThreads) {
       const unsigned long long k = key[i];
       if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
     }
     __syncthreads();
-    if (tid == 0) {
-      int sum = 0, v = 255;
-      for (; v > 0; --v) {
-        if (sum + hist[v] >= want) break;
-        sum += hist[v];
-      }
-      digit = v;
-      above = sum;
+    int total;
+    const int mine = tid < 256 ? hist[255 - tid] : 0;
+    const int before = workgroup_scan(mine, wave_sums, total);
+    if (tid < 256 && before < left && before + mine >= left) {
+      found[0] = 255 - tid;
+      found[1] = before;
     }
     __syncthreads();
-    prefix |= (unsigned long long)digit << shift;
-    want -= above;
+    prefix |= (unsigned long long)found[0] << shift;
+    left -= found[1];
   }
-  // keys above the threshold, and the first `want` that equal it
+  // the blocks at the ends, the keys above the threshold, and the first `left` that equal it
   int done = 0, equal_before = 0;
   for (int i0 = 0; i0 < nb; i0 += kSelectThreads) {
     const int i = i0 + tid;
-    const unsigned long long k = i < nb ? key[i] : 0;
-    const bool eq = i < nb && k == prefix;
+    const bool scored = i >= begin && i < end;
+    const unsigned long long k = scored && want > 0 ? key[i] : 0;
+    const bool eq = scored && want > 0 && k == prefix;
     int total;
     const int rank = equal_before + workgroup_scan(eq, wave_sums, total);
     equal_before += total;
-    const bool take = i < nb && (k > prefix || (eq && rank < want));
+    const bool take = i < nb && (!scored || (want > 0 && (k > prefix || (eq && rank < left))));
     const int at = done + workgroup_scan(take, wave_sums, total);
     done += total;
     if (take) out[at] = i;
@@ -222,21 +642,9 @@ int pa_block_bounds(const PaBlockArgs* a, void* hip_stream) {
     const int64_t reach = ((int64_t)a->new_tokens + a->block_size - 2) / a->block_size + 1;
     if (reach < visits) visits = (int)reach;
   }
-  const int64_t grid = (int64_t)a->num_seqs * visits * a->num_kv_heads;
-  if (grid > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
-  const dim3 g((unsigned)grid), t(64);
-  const bool fp8 = a->kv_dtype == PA_DTYPE_FP8_E4M3FN;
-  switch (a->head_size) {
-    case 64:
-      return fp8 ? pa_launch(pa_block_bounds_kernel<64, true>, g, t, 0, stream, *a, axis, visits)
-                 : pa_launch(pa_block_bounds_kernel<64, false>, g, t, 0, stream, *a, axis, visits);
-    case 128:
-      return fp8 ? pa_launch(pa_block_bounds_kernel<128, true>, g, t, 0, stream, *a, axis, visits)
-                 : pa_launch(pa_block_bounds_kernel<128, false>, g, t, 0, stream, *a, axis, visits);
-    default:
-      return fp8 ? pa_launch(pa_block_bounds_kernel<256, true>, g, t, 0, stream, *a, axis, visits)
-                 : pa_launch(pa_block_bounds_kernel<256, false>, g, t, 0, stream, *a, axis, visits);
-  }
+  return a->head_size == 64    ? launch_bounds<64>(*a, axis, visits, stream)
+         : a->head_size == 128 ? launch_bounds<128>(*a, axis, visits, stream)
+                               : launch_bounds<256>(*a, axis, visits, stream);
 }
 
 int64_t pa_select_blocks_workspace_bytes(const PaBlockArgs* a) {
@@ -251,14 +659,19 @@ int pa_select_blocks(const PaBlockArgs* a, void* hip_stream) {
   if (a->workspace_bytes < need || !block_aligned16(a->workspace)) return PA_ERR_SCRATCH_TOO_SMALL;
   hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
   const int axis = block_axis(*a), blocks = axis_blocks_of(*a);
-  const int64_t grid = (int64_t)a->num_seqs * blocks * a->num_kv_heads;
+  const int64_t heads = (int64_t)a->num_seqs * a->num_kv_heads;
+  // stretches long enough to pay for staging the query, short enough to fill the GPU: 64 blocks up to 2048 workgroups
+  int64_t chunk = (heads * blocks / 2048 + 63) / 64 * 64;
+  chunk = chunk < 64 ? 64 : (chunk > 1024 ? 1024 : chunk);
+  const int64_t grid = heads * ((blocks + chunk - 1) / chunk);
   if (grid > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
-  const dim3 g((unsigned)grid), t(64);
-  const int rc = a->head_size == 64    ? pa_launch(pa_block_score_kernel<64>, g, t, 0, stream, *a, axis, blocks)
-                 : a->head_size == 128 ? pa_launch(pa_block_score_kernel<128>, g, t, 0, stream, *a, axis, blocks)
-                                       : pa_launch(pa_block_score_kernel<256>, g, t, 0, stream, *a, axis, blocks);
+  const dim3 g((unsigned)grid), t(64 * kScoreWaves);
+  const unsigned lds = (unsigned)((a->q_len * a->group_size + 15) / 16) * a->head_size * 64;  // [q-, q+] of 16 rows: 64 D bytes
+  const int rc = a->head_size == 64    ? pa_launch(pa_block_score_kernel<64>, g, t, lds, stream, *a, axis, blocks, (int)chunk)
+                 : a->head_size == 128 ? pa_launch(pa_block_score_kernel<128>, g, t, lds, stream, *a, axis, blocks, (int)chunk)
+                                       : pa_launch(pa_block_score_kernel<256>, g, t, lds, stream, *a, axis, blocks, (int)chunk);
   if (rc) return rc;
-  return pa_launch(pa_block_select_kernel, dim3((unsigned)(a->num_seqs * a->num_kv_heads)), dim3(kSelectThreads), 0, stream, *a, axis, blocks);
+  return pa_launch(pa_block_select_kernel, dim3((unsigned)heads), dim3(kSelectThreads), 0, stream, *a, axis, blocks);
 }
 
 }  // extern "C"

@@ -8,8 +8,9 @@
 // workgroup of the first token of the call that lies in the block: it finds the block's other tokens by reading the
 // whole slot mapping (64 KiB for 8192 tokens, from L2), and no workspace, no sort and no second launch is needed.
 // Per slot the latest token is kept (an LDS maximum of token numbers), so the bytes do not depend on timing.
-// Every byte of the block is written at most once: K in 16-byte (chunk, token) cells, V in 16-byte rows of 16 tokens that
-// mix new codes with old ones.
+// From there on a wave owns a (block, kv head) and needs no barrier: it goes through the block's 16-slot segments that
+// change, 16 bytes of a row per lane.  K leaves as 8-byte halves of (chunk, token) cells, V is turned in LDS so that a
+// head dim's 16 tokens are one 16-byte store, new codes among the old ones.  Every byte is written at most once.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -20,6 +21,7 @@
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 constexpr int kThreads = 256;
 constexpr int kMaxBlockSize = 1024;
@@ -35,7 +37,6 @@ __device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float ratio) {
   return to_codes(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * ratio,
                   __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * ratio);
 }
-__device__ __forceinline__ float bf16_value(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 
 // the smallest power of two s >= 2^-126 with amax <= 448 s, for a bf16 amax given by its bits (finite, sign cleared).
 // 448 = 1.75 * 2^8, so the exponent is that of amax minus 8, plus one if its significand is above 1.75.
@@ -65,144 +66,222 @@ __device__ __forceinline__ u32x4 load_row8(const uint16_t* p) {
   }
 }
 
+// eight codes of x / s for a power of two s = 1 / inv (the product is then the quotient), or any s
+__device__ __forceinline__ u32x2 quantize_row8(u32x4 x, float s, float inv, bool pow2) {
+  u32x2 out;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t p = x[2 * w + (e >> 1)];
+      const float f = __uint_as_float(e & 1 ? p & 0xffff0000u : p << 16);
+      v[e] = pow2 ? f * inv : __fdiv_rn(f, s);
+    }
+    out[w] = to_codes(v[0], v[1], v[2], v[3]);
+  }
+  return out;
+}
+
+// 4x4 transpose of bytes: word i holds byte j of row i, afterwards byte i of column j
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+// One (block, kv head), by one wave.  owner: the block's slots' tokens (LDS); segs: the segments that get a token.
+template <int D, bool ALIGNED>
+__device__ __forceinline__ void write_block_head(const PaKvWriteArgs& a, const long long block, const int h, const int bs, const int* owner,
+                                                 const unsigned long long segs, uint8_t (*turn)[D], const int lane) {
+  constexpr int P = D / 8;         // lanes of a row, 8 head dims each
+  constexpr int R = 16 * P / 64;   // loads per lane for 16 rows
+  constexpr int DL = D / 4;        // lanes that hold four head dims of V each
+  const uint16_t* key = (const uint16_t*)a.key + (int64_t)h * a.stride_k_h + lane % P * 8;
+  const uint16_t* value = (const uint16_t*)a.value + (int64_t)h * a.stride_v_h + lane % P * 8;
+  uint8_t* kc = (uint8_t*)a.key_cache + block * a.stride_kc_b + (int64_t)h * a.stride_kc_h;
+  uint8_t* vc = (uint8_t*)a.value_cache + block * a.stride_vc_b + (int64_t)h * a.stride_vc_h;
+  const int64_t so = block * a.stride_scale_b + (int64_t)h * a.stride_scale_h;
+  const float old_k = a.key_scale[so], old_v = a.value_scale[so];
+
+  u32x4 kr[R], vr[R], was[4];
+  auto token_of = [&](int seg, int j) { return owner[16 * seg + lane / P + 64 / P * j]; };
+  auto load_rows = [&](int seg) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int tok = token_of(seg, j);
+      kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+      if (tok >= 0) {
+        kr[j] = load_row8<ALIGNED>(key + (int64_t)tok * a.stride_k_t);
+        vr[j] = load_row8<ALIGNED>(value + (int64_t)tok * a.stride_v_t);
+      }
+    }
+  };
+  // lane's four head dims 4 lane + i of V: 16 tokens each
+  auto v_row = [&](int seg, int i) {
+    const int d = 4 * lane + i;
+    return reinterpret_cast<u32x4*>(vc + (a.v_transposed ? ((int64_t)seg * D + d) * 16 : (int64_t)d * bs + 16 * seg));
+  };
+  auto member_mask = [&](int seg) {
+    return (uint32_t)__builtin_amdgcn_ballot_w64(owner[16 * seg + (lane & 15)] >= 0) & 0xffffu;
+  };
+  auto load_was = [&](int seg, uint32_t members) {
+    if (members != 0xffffu && lane < DL) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) was[i] = *v_row(seg, i);
+    }
+  };
+
+  // ---- amax of the new rows: the last segment's rows stay in registers ---------------------------------------------------
+  uint32_t mk = 0, mv = 0;
+  int held = -1;
+  for (unsigned long long left = segs; left; left &= left - 1) {
+    held = __builtin_ctzll(left);
+    load_rows(held);
+    if (!(left & (left - 1))) load_was(held, member_mask(held));
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        mk = finite_max2(mk, kr[j][e]);
+        mv = finite_max2(mv, vr[j][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t ok = __shfl_xor(mk, o), ov = __shfl_xor(mv, o);
+    mk = ok > mk ? ok : mk;
+    mv = ov > mv ? ov : mv;
+  }
+  const float new_k = fmaxf(old_k, scale_for(mk)), new_v = fmaxf(old_v, scale_for(mv));
+  const bool grow_k = old_k > 0.f && new_k > old_k, grow_v = old_v > 0.f && new_v > old_v;
+  const float ratio_k = grow_k ? __fdiv_rn(old_k, new_k) : 1.f, ratio_v = grow_v ? __fdiv_rn(old_v, new_v) : 1.f;
+  auto is_pow2 = [](float s) { return (__float_as_uint(s) & 0x7fffffu) == 0 && s >= 0x1p-126f && s <= 0x1p126f; };
+  const bool pow2_k = is_pow2(new_k), pow2_v = is_pow2(new_v);
+  const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
+  if (lane == 0) {
+    a.key_scale[so] = new_k;
+    a.value_scale[so] = new_v;
+  }
+
+  // ---- the segments that change, the one in registers first -----------------------------------------------------------------
+  const unsigned long long all = bs == 1024 ? ~0ull : (1ull << (bs >> 4)) - 1;
+  unsigned long long left = grow_k || grow_v ? all : segs;
+  for (int seg = held; left;) {
+    const uint32_t members = member_mask(seg);
+    if (seg != held) {
+      load_rows(seg);
+      if (members || grow_v) load_was(seg, members);
+    }
+    // K: the lane's 8 head dims of a token are half of a 16-byte (chunk, token) cell
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int slot = 16 * seg + lane / P + 64 / P * j, c = lane % P;
+      if (owner[slot] >= 0)
+        *reinterpret_cast<u32x2*>(kc + ((int64_t)(c >> 1) * bs + slot) * 16 + 8 * (c & 1)) = quantize_row8(kr[j], new_k, inv_k, pow2_k);
+    }
+    if (grow_k) {
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const int cell = lane + 64 * i, slot = 16 * seg + (cell & 15);
+        if (owner[slot] >= 0) continue;
+        u32x4* p = reinterpret_cast<u32x4*>(kc + ((int64_t)(cell >> 4) * bs + slot) * 16);
+        u32x4 w = *p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = rescale_codes(w[e], ratio_k);
+        *p = w;
+      }
+    }
+    // V: codes into LDS as rows, out of it as columns
+    if (members || grow_v) {
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        *reinterpret_cast<u32x2*>(&turn[lane / P + 64 / P * j][lane % P * 8]) = quantize_row8(vr[j], new_v, inv_v, pow2_v);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      if (lane < DL) {
+        u32x4 out[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // tokens 4 e .. 4 e + 3
+          uint32_t w[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint32_t*>(&turn[4 * e + t][4 * lane]);
+          transpose4(w);
+          const uint32_t m = members >> (4 * e) & 15u;  // bytes that are new
+          const uint32_t take = (m & 1 ? 0xffu : 0u) | (m & 2 ? 0xff00u : 0u) | (m & 4 ? 0xff0000u : 0u) | (m & 8 ? 0xff000000u : 0u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o = 0;
+            if (members != 0xffffu) o = grow_v ? rescale_codes(was[i][e], ratio_v) : was[i][e];
+            out[i][e] = (w[i] & take) | (o & ~take);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *v_row(seg, i) = out[i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    left &= ~(1ull << seg);
+    seg = left ? __builtin_ctzll(left) : 0;
+  }
+}
+
 // grid: (windows of `window` tokens) x (groups of `heads` kv heads).  ALIGNED: the rows can be read 16 bytes at a time.
 template <int D, bool ALIGNED>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_block_scaled_kernel(const PaKvWriteArgs a, const long long num_slots,
                                                                                const int bs_shift, const int window, const int heads) {
-  __shared__ int owner[kMaxBlockSize];             // per slot of the block: the latest token of the call, -1 without one
-  __shared__ uint16_t member[kMaxBlockSize];       // the slots that get a token, in any order
-  __shared__ int count, earlier;
-  __shared__ unsigned long long segments;          // bit i: 16-slot segment i gets a token
-  __shared__ uint32_t amax[2];
-  const int tid = threadIdx.x;
-  const int bs = 1 << bs_shift, nseg = bs >> 4;
+  __shared__ int owner[kMaxBlockSize];     // per slot of the block: the latest token of the call, -1 without one
+  __shared__ unsigned long long segments;  // bit i: 16-slot segment i gets a token
+  __shared__ int earlier;
+  __shared__ __attribute__((aligned(16))) uint8_t turn[kThreads / 64][16][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bs = 1 << bs_shift;
   const int num_tokens = (int)a.num_tokens;
   const int head_groups = (a.num_kv_heads + heads - 1) / heads;
   const int h0 = (int)(blockIdx.x % (unsigned)head_groups) * heads;
   const int h1 = h0 + heads < a.num_kv_heads ? h0 + heads : a.num_kv_heads;
   const long long t0 = (long long)(blockIdx.x / (unsigned)head_groups) * window;
-  const long long t_end = t0 + window < num_tokens ? t0 + window : num_tokens;
+  const int t_end = (int)(t0 + window < num_tokens ? t0 + window : num_tokens);
 
-  auto block_of = [&](long long t) -> long long {
-    const long long slot = a.slot_mapping[t];
-    return slot < 0 || slot >= num_slots ? -1 : slot >> bs_shift;
-  };
-  for (int t = (int)t0; t < t_end; ++t) {
-    const long long block = block_of(t);
-    if (block < 0 || (t > 0 && block_of(t - 1) == block)) continue;  // (most tokens of a prompt: their run began earlier)
+  auto block_of = [&](long long slot) -> long long { return slot < 0 || slot >= num_slots ? -1 : slot >> bs_shift; };
+  // the tokens of the window that begin a run in their block (most tokens of a prompt do not)
+  const int mine = (int)t0 + lane;
+  bool begins = false;
+  if (lane < window && mine < t_end) {
+    const long long block = block_of(a.slot_mapping[mine]);
+    begins = block >= 0 && (mine == 0 || block_of(a.slot_mapping[mine - 1]) != block);
+  }
+  for (uint64_t todo = __builtin_amdgcn_ballot_w64(begins); todo; todo &= todo - 1) {
+    const int t = (int)t0 + __builtin_ctzll(todo);
+    const long long block = a.slot_mapping[t] >> bs_shift;
     __syncthreads();  // the previous block's lists are done with
     for (int i = tid; i < bs; i += kThreads) owner[i] = -1;
     if (tid == 0) {
-      count = earlier = 0;
+      earlier = 0;
       segments = 0;
     }
     __syncthreads();
+#pragma unroll 8
     for (int i = tid; i < num_tokens; i += kThreads) {
       const long long slot = a.slot_mapping[i];
-      if (slot < 0 || slot >= num_slots || slot >> bs_shift != block) continue;
-      if (i < t)
+      if (block_of(slot) != block) continue;
+      if (i < t) {
         earlier = 1;
-      else
+      } else {
         atomicMax(&owner[slot & (bs - 1)], i);
+        atomicOr(&segments, 1ull << ((slot & (bs - 1)) >> 4));
+      }
     }
     __syncthreads();
     if (earlier) continue;  // another workgroup (or an earlier turn of this one) owns the block
-    for (int i = tid; i < bs; i += kThreads) {
-      if (owner[i] < 0) continue;
-      member[atomicAdd(&count, 1)] = (uint16_t)i;
-      atomicOr(&segments, 1ull << (i >> 4));
-    }
-    __syncthreads();
-    const int n = count;
-    const unsigned long long segs = segments;
-
-    for (int h = h0; h < h1; ++h) {
-      const uint16_t* key = (const uint16_t*)a.key + (int64_t)h * a.stride_k_h;
-      const uint16_t* value = (const uint16_t*)a.value + (int64_t)h * a.stride_v_h;
-      // ---- amax of the new rows -----------------------------------------------------------------------------------
-      if (tid < 2) amax[tid] = 0;
-      __syncthreads();
-      uint32_t mk = 0, mv = 0;
-      for (int i = tid; i < n * (D / 8); i += kThreads) {
-        const int64_t tok = owner[member[i / (D / 8)]];
-        const int d = i % (D / 8) * 8;
-        const u32x4 k8 = load_row8<ALIGNED>(key + tok * a.stride_k_t + d), v8 = load_row8<ALIGNED>(value + tok * a.stride_v_t + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          mk = finite_max2(mk, k8[e]);
-          mv = finite_max2(mv, v8[e]);
-        }
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t ok = __shfl_xor(mk, o), ov = __shfl_xor(mv, o);
-        mk = ok > mk ? ok : mk;
-        mv = ov > mv ? ov : mv;
-      }
-      if ((tid & 63) == 0) {
-        atomicMax(&amax[0], mk);
-        atomicMax(&amax[1], mv);
-      }
-      // every thread reads the old scales before the barrier that lets thread 0 write the new ones
-      const int64_t so = block * a.stride_scale_b + (int64_t)h * a.stride_scale_h;
-      const float old_k = a.key_scale[so], old_v = a.value_scale[so];
-      __syncthreads();
-      const float new_k = fmaxf(old_k, scale_for(amax[0])), new_v = fmaxf(old_v, scale_for(amax[1]));
-      const bool grow_k = old_k > 0.f && new_k > old_k, grow_v = old_v > 0.f && new_v > old_v;
-      const float ratio_k = grow_k ? __fdiv_rn(old_k, new_k) : 1.f, ratio_v = grow_v ? __fdiv_rn(old_v, new_v) : 1.f;
-      if (tid == 0) {
-        a.key_scale[so] = new_k;
-        a.value_scale[so] = new_v;
-      }
-      // ---- K: 16-byte cells (16 head dims of a token) --------------------------------------------------------------------
-      uint8_t* kc = (uint8_t*)a.key_cache + block * a.stride_kc_b + (int64_t)h * a.stride_kc_h;
-      for (int i = tid; i < n * (D / 16); i += kThreads) {
-        const int off = member[i / (D / 16)], c = i % (D / 16);
-        const uint16_t* row = key + (int64_t)owner[off] * a.stride_k_t + 16 * c;
-        const u32x4 x0 = load_row8<ALIGNED>(row), x1 = load_row8<ALIGNED>(row + 8);
-        u32x4 out;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t p = w < 2 ? x0[2 * w] : x1[2 * w - 4], q = w < 2 ? x0[2 * w + 1] : x1[2 * w - 3];
-          out[w] = to_codes(__fdiv_rn(bf16_value(p & 0xffffu), new_k), __fdiv_rn(bf16_value(p >> 16), new_k),
-                            __fdiv_rn(bf16_value(q & 0xffffu), new_k), __fdiv_rn(bf16_value(q >> 16), new_k));
-        }
-        *reinterpret_cast<u32x4*>(kc + ((int64_t)c * bs + off) * 16) = out;
-      }
-      if (grow_k) {
-        for (int i = tid; i < bs * (D / 16); i += kThreads) {
-          if (owner[i & (bs - 1)] >= 0) continue;
-          u32x4* p = reinterpret_cast<u32x4*>(kc + (int64_t)i * 16);
-          u32x4 w = *p;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = rescale_codes(w[e], ratio_k);
-          *p = w;
-        }
-      }
-      // ---- V: 16 tokens of a head dim, new codes among the old ones ---------------------------------------------------------
-      uint8_t* vc = (uint8_t*)a.value_cache + block * a.stride_vc_b + (int64_t)h * a.stride_vc_h;
-      constexpr int kSegs = kThreads / D;  // segments the workgroup takes at a time, D threads each
-      const int d = tid % D;
-      for (int seg = tid / D; seg < nseg; seg += kSegs) {
-        if (!grow_v && !((segs >> seg) & 1)) continue;
-        u32x4* p = reinterpret_cast<u32x4*>(vc + (a.v_transposed ? ((int64_t)seg * D + d) * 16 : (int64_t)d * bs + 16 * seg));
-        u32x4 w = *p;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (grow_v) w[e] = rescale_codes(w[e], ratio_v);
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int tok = owner[16 * seg + 4 * e + b];
-            if (tok < 0) continue;
-            const float x = bf16_value(value[(int64_t)tok * a.stride_v_t + d]);
-            const uint32_t code = to_codes(__fdiv_rn(x, new_v), 0.f, 0.f, 0.f) & 0xffu;
-            w[e] = (w[e] & ~(0xffu << (8 * b))) | (code << (8 * b));
-          }
-        }
-        *p = w;
-      }
-      __syncthreads();  // amax is free for the next head
-    }
+    for (int h = h0 + wave; h < h1; h += kThreads / 64) write_block_head<D, ALIGNED>(a, block, h, bs, owner, segments, turn[wave], lane);
   }
 }
 
@@ -223,10 +302,10 @@ extern "C" int pa_kv_cache_write_block_scaled(const PaKvWriteArgs* a, int64_t nu
   if ((caches & 15) || a->stride_kc_b % 16 || a->stride_kc_h % 16 || a->stride_vc_b % 16 || a->stride_vc_h % 16) return PA_ERR_BAD_SHAPE;
   const uintptr_t rows = reinterpret_cast<uintptr_t>(a->key) | reinterpret_cast<uintptr_t>(a->value);
   const bool aligned = (rows & 15) == 0 && a->stride_k_t % 8 == 0 && a->stride_k_h % 8 == 0 && a->stride_v_t % 8 == 0 && a->stride_v_h % 8 == 0;
-  // a few tokens (decode): one workgroup per (token, kv head).  Many (prompts): most tokens own no block, so a
+  // A few tokens (decode): one workgroup per (token, four kv heads).  Many (prompts): most tokens own no block, so a
   // workgroup looks at 16 of them, and walks all kv heads so that the slot mapping is read once per block.
   const bool many = a->num_tokens > 1024;
-  const int window = many ? 16 : 1, heads = many ? a->num_kv_heads : 1;
+  const int window = many ? 16 : 1, heads = many ? a->num_kv_heads : kThreads / 64;
   const int64_t grid = ((a->num_tokens + window - 1) / window) * ((a->num_kv_heads + heads - 1) / heads);
   if (grid > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
   const int shift = __builtin_ctz((unsigned)a->block_size);
