@@ -13,75 +13,80 @@ read nothing back to the host and can be captured into a graph; there is no torc
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _cabi
 from ._cabi import PaBlockArgs
-from .kv_cache import FP8_DTYPE
+from .kv_cache import FP8_DTYPE, _current_raw_stream, _strides
 
 _SUPPORTED_BLOCK_SIZES = (16, 64, 1024)
 _SUPPORTED_HEAD_SIZES = (64, 128, 256)
 
-
-def _on(dev: torch.device):
-    """The context in which a launch on `dev` is made: nothing when it is the current device already."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
-
-
-def _strides(t: torch.Tensor) -> Tuple[int, ...]:
-    """Strides with 0 for a dimension of size 1, whose stride means nothing."""
-    return tuple(st if n > 1 else 0 for n, st in zip(t.shape, t.stride()))
+# PaBlockArgs in one go, in the order of its fields (filling some 50 attributes of a ctypes structure takes longer than
+# the kernels of a small call)
+_PACK = struct.Struct("<Ii14Q16ifi20q")
+_SIZE = C.sizeof(PaBlockArgs)
+assert _PACK.size == _SIZE
 
 
-def _same_device(dev, **tensors) -> None:
+def _check_devices(index: int, dev: torch.device, tensors: dict) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
+        if t is not None and (t.get_device() != index or (index < 0 and t.device != dev)):
             raise ValueError(f"{name} is on {t.device}, the call on {dev}")
 
 
-def _check_sequences(a: PaBlockArgs, sequence_lengths, block_tables, max_sequence_length) -> None:
-    if sequence_lengths.dtype != torch.int32 or block_tables.dtype != torch.int32:
+def _launch(name: str, args: PaBlockArgs, index: int, stream: Optional[int] = None) -> None:
+    """Calls an entry point of the library on torch's current stream of device `index`, with that device current."""
+    if index == torch.cuda.current_device():
+        if stream is None:
+            stream = _current_raw_stream(index)
+        rc = getattr(_cabi.load_library(), name)(C.byref(args), stream)
+        if rc:
+            _cabi.check(rc, name)
+    else:
+        with torch.cuda.device(index):
+            _launch(name, args, index, stream)
+
+
+def _check_sequences(lens, tables) -> Tuple[int, int, int]:
+    """(number of sequences, entries of a table row, stride of the rows)"""
+    if lens.dtype is not torch.int32 or tables.dtype is not torch.int32:
         raise ValueError("sequence_lengths and block_tables must be int32")
-    if block_tables.dim() != 2 or sequence_lengths.numel() != block_tables.shape[0] or block_tables.shape[1] < 1:
+    shape = tables.shape
+    if len(shape) != 2 or lens.numel() != shape[0] or shape[1] < 1:
         raise ValueError("sequence_lengths / block_tables do not have one row per sequence")
-    if not sequence_lengths.is_contiguous() or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    row, col = tables.stride()
+    if not lens.is_contiguous() or (col != 1 and shape[1] > 1):
         raise ValueError("sequence_lengths and the rows of block_tables must be contiguous")
-    a.context_lens, a.block_tables = sequence_lengths.data_ptr(), block_tables.data_ptr()
-    a.num_seqs, a.table_width = block_tables.shape
-    a.stride_bt_s = block_tables.stride(0)
-    a.max_context_len = max(0, int(max_sequence_length))
+    return shape[0], shape[1], row
 
 
-def _check_query(a: PaBlockArgs, query, query_sequence_length, num_kv_heads, query_lens) -> None:
+def _check_query(query, q_len: int, num_kv_heads: int, num_seqs: int, query_lens) -> Tuple[int, int, int, int]:
+    """(query rows per kv head and new token, head size, strides)"""
     if query.dim() != 3:
         raise ValueError(f"Expected 3D query tensor, but got shape {tuple(query.shape)}")
-    if query.dtype != torch.bfloat16:
+    if query.dtype is not torch.bfloat16:
         raise ValueError(f"query tensor only supports dtype bfloat16, but got {query.dtype}")
-    q_len = int(query_sequence_length)
-    num_seqs, rows, head_size = query.shape
+    seqs, rows, head_size = query.shape
     if q_len < 1 or rows == 0 or rows % (q_len * num_kv_heads):
         raise ValueError(f"query.shape[1]={rows} is not num_kv_heads*query_sequence_length*group ({num_kv_heads}*{q_len}*G)")
     if rows // num_kv_heads > 64:
         raise ValueError(f"{rows // num_kv_heads} query rows per kv head exceed the maximum of 64")
-    if num_seqs != a.num_seqs:
+    if seqs != num_seqs:
         raise ValueError("sequence_lengths / block_tables do not have one row per sequence")
     if head_size not in _SUPPORTED_HEAD_SIZES:
         raise ValueError(f"head_size == {head_size} is not supported (64, 128 or 256)")
-    if query.stride(2) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.data_ptr() % 16:
+    st = query.stride()
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or query.data_ptr() % 16:
         raise ValueError("query rows must be dense and 16-byte aligned")
-    if query_lens is not None:
-        if query_lens.dtype != torch.int32 or query_lens.numel() != num_seqs or not query_lens.is_contiguous():
-            raise ValueError("query_lens must be contiguous int32 [num_seqs]")
-        a.q_lens = query_lens.data_ptr()
-    a.query = query.data_ptr()
-    a.q_len, a.group_size, a.head_size = q_len, rows // (q_len * num_kv_heads), head_size
-    a.stride_q_s, a.stride_q_h = query.stride(0), query.stride(1)
+    if query_lens is not None and (query_lens.dtype is not torch.int32 or query_lens.numel() != seqs or not query_lens.is_contiguous()):
+        raise ValueError("query_lens must be contiguous int32 [num_seqs]")
+    return rows // (q_len * num_kv_heads), head_size, st[0], st[1]
 
 
 def _check_block_size(block_size: int) -> None:
@@ -89,69 +94,102 @@ def _check_block_size(block_size: int) -> None:
         raise ValueError(f"kv_block_size == {block_size} not in {list(_SUPPORTED_BLOCK_SIZES)}")
 
 
-def _check_key_cache(a: PaBlockArgs, key_cache) -> None:
-    if key_cache.dim() != 5:
-        raise ValueError(f"Expected 5D key_cache tensor, but got shape {tuple(key_cache.shape)}")
-    if key_cache.dtype == FP8_DTYPE:
-        a.kv_dtype, x = _cabi.PA_DTYPE_FP8_E4M3FN, 16
-    elif key_cache.dtype == torch.bfloat16:
-        a.kv_dtype, x = _cabi.PA_DTYPE_BF16, 8
+def _check_key_cache(key_cache):
+    """(dtype code, elements per 16 bytes, blocks, kv heads, block size, head size, strides of the first three dimensions)"""
+    shape = key_cache.shape
+    if len(shape) != 5:
+        raise ValueError(f"Expected 5D key_cache tensor, but got shape {tuple(shape)}")
+    if key_cache.dtype is FP8_DTYPE:
+        code, x = _cabi.PA_DTYPE_FP8_E4M3FN, 16
+    elif key_cache.dtype is torch.bfloat16:
+        code, x = _cabi.PA_DTYPE_BF16, 8
     else:
         raise ValueError(f"key_cache tensor only supports dtype bfloat16 or float8_e4m3fn, but got {key_cache.dtype}")
-    blocks, heads, chunks, bs, inner = key_cache.shape
+    blocks, heads, chunks, bs, inner = shape
     _check_block_size(bs)
     if inner != x or chunks * x not in _SUPPORTED_HEAD_SIZES or blocks < 1 or heads < 1:
-        raise ValueError(f"key_cache shape {tuple(key_cache.shape)} is not [blocks, kv_heads, head_size//{x}, bs, {x}] "
+        raise ValueError(f"key_cache shape {tuple(shape)} is not [blocks, kv_heads, head_size//{x}, bs, {x}] "
                          "with a head size of 64, 128 or 256")
-    st = key_cache.stride()
-    if st[4] != 1 or st[3] != x or st[0] % x or st[1] % x or st[2] % x or key_cache.data_ptr() % 16:
+    s0, s1, s2, s3, s4 = key_cache.stride()
+    if s4 != 1 or s3 != x or s0 % x or s1 % x or s2 % x or key_cache.data_ptr() % 16:
         raise ValueError("the innermost dimensions of key_cache must be dense and 16-byte aligned")
-    a.key_cache = key_cache.data_ptr()
-    a.num_blocks, a.num_kv_heads, a.block_size, a.head_size = blocks, heads, bs, chunks * x
-    a.stride_k_b, a.stride_k_h, a.stride_k_c = st[0], st[1], st[2]
+    return code, x, blocks, heads, bs, chunks * x, s0, s1, s2
 
 
-def _check_scales(a: PaBlockArgs, key_scale, value_scale, both: bool) -> None:
-    a.kv_quant_mode = _cabi.PA_QUANT_NONE
+def _check_scales(code: int, blocks: int, heads: int, bs: int, key_scale, value_scale, both: bool) -> Tuple[int, int, int]:
+    """(quantisation mode, strides over blocks and heads)"""
     if both and (key_scale is None) != (value_scale is None):
         raise ValueError("key_scale and value_scale must be given together")
     if key_scale is None:
-        return
-    if a.kv_dtype != _cabi.PA_DTYPE_FP8_E4M3FN:
+        return _cabi.PA_QUANT_NONE, 0, 0
+    if code != _cabi.PA_DTYPE_FP8_E4M3FN:
         raise ValueError("scales need an FP8 cache")
-    for name, s in (("key_scale", key_scale), ("value_scale", value_scale)):
-        if s is not None and s.dtype != torch.float32:
-            raise ValueError(f"{name} tensor only support dtype == torch.float32")
-    if both and (key_scale.shape != value_scale.shape or _strides(key_scale) != _strides(value_scale)):
-        raise ValueError("key and value scales must have the same shape and strides")
+    if key_scale.dtype is not torch.float32 or (both and value_scale.dtype is not torch.float32):
+        raise ValueError("key_scale / value_scale tensors only support dtype == torch.float32")
     shape = tuple(key_scale.shape)
+    if both and (shape != tuple(value_scale.shape) or (key_scale.stride() != value_scale.stride() and _strides(key_scale) != _strides(value_scale))):
+        raise ValueError("key and value scales must have the same shape and strides")
     if shape == ():
-        a.kv_quant_mode = _cabi.PA_QUANT_PER_TENSOR
-    elif shape == (a.num_blocks, a.num_kv_heads, 1, 1):
-        a.kv_quant_mode = _cabi.PA_QUANT_PER_BLOCK
-    elif shape == (a.num_blocks, a.num_kv_heads, a.block_size, 1):
-        if key_scale.stride(2) != 1 or key_scale.stride(0) % 4 or key_scale.stride(1) % 4 or key_scale.data_ptr() % 16 or \
-                (both and value_scale.data_ptr() % 16):
-            raise ValueError("per-token scales must be dense over tokens and 16-byte aligned")
-        a.kv_quant_mode = _cabi.PA_QUANT_PER_TOKEN
-    else:
-        raise ValueError(f"Expected scales of shape [], [{a.num_blocks}, {a.num_kv_heads}, 1, 1] or "
-                         f"[{a.num_blocks}, {a.num_kv_heads}, {a.block_size}, 1], got {shape}")
-    if shape:
-        a.stride_kvscale_b, a.stride_kvscale_h = key_scale.stride(0), key_scale.stride(1)
-    a.key_scale = key_scale.data_ptr()
-    if both:
-        a.value_scale = value_scale.data_ptr()
+        return _cabi.PA_QUANT_PER_TENSOR, 0, 0
+    st = key_scale.stride()
+    if shape == (blocks, heads, 1, 1):
+        return _cabi.PA_QUANT_PER_BLOCK, st[0], st[1]
+    if shape != (blocks, heads, bs, 1):
+        raise ValueError(f"Expected scales of shape [], [{blocks}, {heads}, 1, 1] or [{blocks}, {heads}, {bs}, 1], got {shape}")
+    if st[2] != 1 or st[0] % 4 or st[1] % 4 or key_scale.data_ptr() % 16 or (both and value_scale.data_ptr() % 16):
+        raise ValueError("per-token scales must be dense over tokens and 16-byte aligned")
+    return _cabi.PA_QUANT_PER_TOKEN, st[0], st[1]
 
 
-def _check_bounds(a: PaBlockArgs, bounds) -> None:
-    if bounds.dtype != torch.bfloat16 or bounds.dim() != 4 or bounds.shape[2] != 2:
+def _check_bounds(bounds) -> Tuple[int, int]:
+    """strides over blocks and heads"""
+    shape = bounds.shape
+    if bounds.dtype is not torch.bfloat16 or len(shape) != 4 or shape[2] != 2:
         raise ValueError("bounds must be bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
-    st = bounds.stride()
-    if st[3] != 1 or st[2] != bounds.shape[3] or st[0] % 8 or st[1] % 8 or bounds.data_ptr() % 16:
+    s0, s1, s2, s3 = bounds.stride()
+    if s3 != 1 or s2 != shape[3] or s0 % 8 or s1 % 8 or bounds.data_ptr() % 16:
         raise ValueError("the two bounds of a (block, head) must be dense and 16-byte aligned")
-    a.bounds = bounds.data_ptr()
-    a.stride_bounds_b, a.stride_bounds_h = st[0], st[1]
+    return s0, s1
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(num_seqs, heads, group, q_len, head_size, bs, width, longest, num_selected) -> int:
+    """pa_block_attention_workspace_bytes, a pure function of these sizes."""
+    aligned = 1 << 12  # (an address that passes the library's checks and is not followed)
+    a = PaBlockArgs(struct_size=_SIZE, output=aligned, query=aligned, key_cache=aligned, value_cache=aligned, context_lens=aligned,
+                    block_tables=aligned, num_seqs=num_seqs, num_kv_heads=heads, group_size=group, q_len=q_len, head_size=head_size,
+                    block_size=bs, num_blocks=1, table_width=width, max_context_len=longest, kv_quant_mode=_cabi.PA_QUANT_NONE,
+                    selected_blocks=aligned if num_selected else None, num_selected=num_selected)
+    return _workspace_bytes("pa_block_attention_workspace_bytes", a)
+
+
+@functools.lru_cache(maxsize=4096)
+def _select_workspace(num_seqs, heads, group, q_len, head_size, bs, width, longest) -> int:
+    """pa_select_blocks_workspace_bytes, a pure function of these sizes."""
+    aligned = 1 << 12
+    a = PaBlockArgs(struct_size=_SIZE, query=aligned, context_lens=aligned, block_tables=aligned, bounds=aligned, selected_blocks=aligned,
+                    selected_counts=aligned, num_seqs=num_seqs, num_kv_heads=heads, group_size=group, q_len=q_len, head_size=head_size,
+                    block_size=bs, num_blocks=1, table_width=width, max_context_len=longest, num_selected=1)
+    return _workspace_bytes("pa_select_blocks_workspace_bytes", a)
+
+
+def _workspace_bytes(name: str, a: PaBlockArgs) -> int:
+    need = getattr(_cabi.load_library(), name)(C.byref(a))
+    if need < 0:
+        _cabi.check(int(need), name)
+    return need
+
+
+def _give_workspace(workspace, need: int, dev) -> Optional[torch.Tensor]:
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16:
+        raise ValueError(f"workspace must be a contiguous, 16-byte aligned uint8 tensor of at least {need} bytes")
+    return workspace
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 class BlockAttentionPlan:
@@ -161,16 +199,11 @@ class BlockAttentionPlan:
 
     def __init__(self, args: PaBlockArgs, keep, output):
         self.args, self._keep, self.output = args, keep, output
-        self._lib = _cabi.load_library()
+        self._index = output.get_device()
 
     def run(self, stream: Optional[int] = None) -> None:
-        if not self.args.num_seqs:
-            return
-        dev = self.output.device
-        with _on(dev):
-            if stream is None:
-                stream = torch.cuda.current_stream(dev).cuda_stream
-            _cabi.check(self._lib.pa_block_attention(C.byref(self.args), C.c_void_p(stream)), "pa_block_attention")
+        if self.args.num_seqs:
+            _launch("pa_block_attention", self.args, self._index, stream)
 
 
 def plan_block_attention(
@@ -192,86 +225,70 @@ def plan_block_attention(
     lse: Optional[torch.Tensor] = None,              # [num_seqs, rows] f32, written
     workspace: Optional[torch.Tensor] = None,        # uint8
 ) -> BlockAttentionPlan:
-    a = PaBlockArgs()
-    a.struct_size = C.sizeof(PaBlockArgs)
-    dev = output.device
-    _same_device(dev, query=query, key_cache=key_cache, value_cache=value_cache, sequence_lengths=sequence_lengths,
-                 block_tables=block_tables, key_scale=key_scale, value_scale=value_scale, selected_blocks=selected_blocks,
-                 selected_counts=selected_counts, query_lens=query_lens, lse=lse, workspace=workspace)
-    _check_sequences(a, sequence_lengths, block_tables, max_sequence_length)
-    _check_key_cache(a, key_cache)
-    head_size, bs, heads = a.head_size, a.block_size, a.num_kv_heads
-    _check_query(a, query, query_sequence_length, heads, query_lens)
-    if a.head_size != head_size:
-        raise ValueError(f"query has head size {a.head_size}, key_cache {head_size}")
-    if output.shape != query.shape or output.dtype != torch.bfloat16:
+    dev, index = output.device, output.get_device()
+    _check_devices(index, dev, dict(
+        query=query, key_cache=key_cache, value_cache=value_cache, sequence_lengths=sequence_lengths, block_tables=block_tables,
+        key_scale=key_scale, value_scale=value_scale, selected_blocks=selected_blocks, selected_counts=selected_counts,
+        query_lens=query_lens, lse=lse, workspace=workspace))
+    num_seqs, width, st_bt = _check_sequences(sequence_lengths, block_tables)
+    code, x, blocks, heads, bs, head_size, st_kb, st_kh, st_kc = _check_key_cache(key_cache)
+    q_len, longest = int(query_sequence_length), max(0, int(max_sequence_length))
+    group, q_head_size, st_qs, st_qh = _check_query(query, q_len, heads, num_seqs, query_lens)
+    if q_head_size != head_size:
+        raise ValueError(f"query has head size {q_head_size}, key_cache {head_size}")
+    if output.shape != query.shape or output.dtype is not torch.bfloat16:
         raise ValueError(f"output must be bfloat16 {tuple(query.shape)}, got {output.dtype} {tuple(output.shape)}")
-    if output.stride(2) != 1 or output.stride(0) % 4 or output.stride(1) % 4 or output.data_ptr() % 8:
+    st_os, st_oh, st_od = output.stride()
+    if st_od != 1 or st_os % 4 or st_oh % 4 or output.data_ptr() % 8:
         raise ValueError("output rows must be dense and 8-byte aligned")
     # ---- value cache ---------------------------------------------------------------------------------------------------
-    x = 16 // key_cache.element_size()
-    if value_cache.dtype != key_cache.dtype:
+    if value_cache.dtype is not key_cache.dtype:
         raise ValueError(f"value_cache dtype {value_cache.dtype} differs from key_cache dtype {key_cache.dtype}")
-    a.v_transposed = int(value_cache.dim() == 5)
-    inner = (bs // x, head_size, x) if a.v_transposed else (head_size, bs)
-    if tuple(value_cache.shape) != (a.num_blocks, heads) + inner:
+    v_transposed = value_cache.dim() == 5
+    if value_cache.shape != ((blocks, heads, bs // x, head_size, x) if v_transposed else (blocks, heads, head_size, bs)):
         raise ValueError(f"value_cache shape {tuple(value_cache.shape)} is not [blocks, kv_heads, D, bs] or, transposed, "
                          f"[blocks, kv_heads, bs/{x}, D, {x}] of the key cache")
-    st = value_cache.stride()
-    if st[-1] != 1 or (a.v_transposed and st[3] != x) or any(s % x for s in st[:3]) or value_cache.data_ptr() % 16:
+    st_v = value_cache.stride()
+    if st_v[-1] != 1 or (v_transposed and st_v[3] != x) or st_v[0] % x or st_v[1] % x or st_v[2] % x or value_cache.data_ptr() % 16:
         raise ValueError("the innermost dimensions of value_cache must be dense and 16-byte aligned")
-    a.value_cache = value_cache.data_ptr()
-    a.stride_v_b, a.stride_v_h, a.stride_v_2 = st[0], st[1], st[2]
-    _check_scales(a, key_scale, value_scale, True)
+    mode, st_sb, st_sh = _check_scales(code, blocks, heads, bs, key_scale, value_scale, True)
     # ---- the list ----------------------------------------------------------------------------------------------------------
+    num_selected = st_ls = st_lh = st_cs = st_lse = 0
     if selected_blocks is not None:
-        if selected_blocks.dtype != torch.int32 or selected_blocks.dim() != 3 or \
-                tuple(selected_blocks.shape[:2]) != (a.num_seqs, heads) or selected_blocks.shape[2] < 1:
-            raise ValueError(f"selected_blocks must be int32 [{a.num_seqs}, {heads}, k]")
-        if selected_blocks.shape[2] > 1 and selected_blocks.stride(2) != 1:
+        shape = selected_blocks.shape
+        if selected_blocks.dtype is not torch.int32 or len(shape) != 3 or shape[0] != num_seqs or shape[1] != heads or shape[2] < 1:
+            raise ValueError(f"selected_blocks must be int32 [{num_seqs}, {heads}, k]")
+        num_selected = shape[2]
+        st_ls, st_lh, st_lk = selected_blocks.stride()
+        if num_selected > 1 and st_lk != 1:
             raise ValueError("selected_blocks must be contiguous in its last dimension")
-        a.selected_blocks, a.num_selected = selected_blocks.data_ptr(), selected_blocks.shape[2]
-        a.stride_sel_s, a.stride_sel_h = selected_blocks.stride(0), selected_blocks.stride(1)
     if selected_counts is not None:
         if selected_blocks is None:
             raise ValueError("selected_counts needs selected_blocks")
-        if selected_counts.dtype != torch.int32 or tuple(selected_counts.shape) != (a.num_seqs, heads) or \
-                (heads > 1 and selected_counts.stride(1) != 1):
-            raise ValueError(f"selected_counts must be int32 [{a.num_seqs}, {heads}], dense over the heads")
-        a.selected_counts, a.stride_cnt_s = selected_counts.data_ptr(), selected_counts.stride(0)
+        if selected_counts.dtype is not torch.int32 or selected_counts.shape != (num_seqs, heads) or (heads > 1 and selected_counts.stride(1) != 1):
+            raise ValueError(f"selected_counts must be int32 [{num_seqs}, {heads}], dense over the heads")
+        st_cs = selected_counts.stride(0)
     if lse is not None:
-        if lse.dtype != torch.float32 or tuple(lse.shape) != tuple(query.shape[:2]) or lse.stride(1) != 1:
+        if lse.dtype is not torch.float32 or lse.shape != query.shape[:2] or lse.stride(1) != 1:
             raise ValueError(f"lse must be float32 {tuple(query.shape[:2])}, dense over the rows")
-        a.lse, a.stride_lse_s = lse.data_ptr(), lse.stride(0)
-    a.output = output.data_ptr()
-    a.stride_out_s, a.stride_out_h = output.stride(0), output.stride(1)
-    a.softmax_scale = float(softmax_scale)
+        st_lse = lse.stride(0)
     if not output.is_cuda:
         raise ValueError("paged_block_attention runs on the GPU only (there is no CPU path); got a CPU tensor")
+    if num_seqs:
+        need = _attention_workspace(num_seqs, heads, group, q_len, head_size, bs, width, longest, num_selected)
+        workspace = _give_workspace(workspace, need, dev)
+    args = PaBlockArgs.from_buffer_copy(_PACK.pack(
+        _SIZE, 0,
+        output.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scale), _ptr(value_scale),
+        sequence_lengths.data_ptr(), block_tables.data_ptr(), _ptr(query_lens), 0, _ptr(selected_blocks), _ptr(selected_counts), _ptr(lse),
+        _ptr(workspace),
+        num_seqs, heads, group, q_len, head_size, bs, blocks, width, longest, code, mode, v_transposed, num_selected, 0, 0, 0,
+        softmax_scale, 0,
+        st_os, st_oh, st_qs, st_qh, st_kb, st_kh, st_kc, st_v[0], st_v[1], st_v[2], st_sb, st_sh, st_bt, 0, 0,
+        st_ls, st_lh, st_cs, st_lse, 0 if workspace is None else workspace.numel()))
     keep = (output, query, key_cache, value_cache, sequence_lengths, block_tables, key_scale, value_scale,
-            selected_blocks, selected_counts, query_lens, lse)
-    if a.num_seqs:
-        need = _workspace_bytes("pa_block_attention_workspace_bytes", a)
-        keep += (_give_workspace(a, workspace, need, dev),)
-    return BlockAttentionPlan(a, keep, output)
-
-
-def _workspace_bytes(name: str, a: PaBlockArgs) -> int:
-    need = getattr(_cabi.load_library(), name)(C.byref(a))
-    if need < 0:
-        _cabi.check(int(need), name)
-    return need
-
-
-def _give_workspace(a: PaBlockArgs, workspace, need: int, dev) -> Optional[torch.Tensor]:
-    if workspace is None:
-        if need == 0:
-            return None
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16:
-        raise ValueError(f"workspace must be a contiguous, 16-byte aligned uint8 tensor of at least {need} bytes")
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    return workspace
+            selected_blocks, selected_counts, query_lens, lse, workspace)
+    return BlockAttentionPlan(args, keep, output)
 
 
 def paged_block_attention(
@@ -321,26 +338,27 @@ def key_block_bounds(
     length, rounded to bf16; NaN keys are passed over.  `new_tokens` visits only the blocks that hold each sequence's
     last so many tokens (a decode step); other blocks keep their bounds.  A block that stands in several rows has to be
     as full in each of them as far as it is visited (shared prefixes are whole blocks)."""
-    a = PaBlockArgs()
-    a.struct_size = C.sizeof(PaBlockArgs)
-    dev = bounds.device
-    _same_device(dev, key_cache=key_cache, sequence_lengths=sequence_lengths, block_tables=block_tables, key_scale=key_scale)
-    _check_sequences(a, sequence_lengths, block_tables, max_sequence_length)
-    _check_key_cache(a, key_cache)
-    _check_scales(a, key_scale, None, False)
-    _check_bounds(a, bounds)
-    if tuple(bounds.shape) != (a.num_blocks, a.num_kv_heads, 2, a.head_size):
-        raise ValueError(f"bounds shape {tuple(bounds.shape)} is not [{a.num_blocks}, {a.num_kv_heads}, 2, {a.head_size}]")
-    if new_tokens is not None:
-        if int(new_tokens) < 1:
-            raise ValueError(f"new_tokens must be positive, got {new_tokens}")
-        a.new_tokens = int(new_tokens)
+    dev, index = bounds.device, bounds.get_device()
+    _check_devices(index, dev, dict(key_cache=key_cache, sequence_lengths=sequence_lengths, block_tables=block_tables, key_scale=key_scale))
+    num_seqs, width, st_bt = _check_sequences(sequence_lengths, block_tables)
+    code, _, blocks, heads, bs, head_size, st_kb, st_kh, st_kc = _check_key_cache(key_cache)
+    mode, st_sb, st_sh = _check_scales(code, blocks, heads, bs, key_scale, None, False)
+    st_bb, st_bh = _check_bounds(bounds)
+    if bounds.shape != (blocks, heads, 2, head_size):
+        raise ValueError(f"bounds shape {tuple(bounds.shape)} is not [{blocks}, {heads}, 2, {head_size}]")
+    new = 0 if new_tokens is None else int(new_tokens)
+    if new_tokens is not None and new < 1:
+        raise ValueError(f"new_tokens must be positive, got {new_tokens}")
     if not bounds.is_cuda:
         raise ValueError("key_block_bounds runs on the GPU only (there is no CPU path); got a CPU tensor")
-    if a.num_seqs:
-        with _on(dev):
-            lib = _cabi.load_library()
-            _cabi.check(lib.pa_block_bounds(C.byref(a), C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "pa_block_bounds")
+    if num_seqs:
+        args = PaBlockArgs.from_buffer_copy(_PACK.pack(
+            _SIZE, 0,
+            0, 0, key_cache.data_ptr(), 0, _ptr(key_scale), 0, sequence_lengths.data_ptr(), block_tables.data_ptr(), 0, bounds.data_ptr(), 0, 0, 0, 0,
+            num_seqs, heads, 0, 0, head_size, bs, blocks, width, max(0, int(max_sequence_length)), code, mode, 0, 0, 0, 0, min(new, 1 << 30),
+            0.0, 0,
+            0, 0, 0, 0, st_kb, st_kh, st_kc, 0, 0, 0, st_sb, st_sh, st_bt, st_bb, st_bh, 0, 0, 0, 0, 0))
+        _launch("pa_block_bounds", args, index)
     return bounds
 
 
@@ -367,49 +385,47 @@ def select_blocks(
     key within the bounds; scores are ranked by their value in 64 bits, ties go to the lower block.  The first
     `first_blocks` and last `recent_blocks` blocks are always taken; `recent_blocks` defaults to, and is at least, the number of
     blocks the new tokens can lie in."""
-    a = PaBlockArgs()
-    a.struct_size = C.sizeof(PaBlockArgs)
-    dev = query.device
-    _same_device(dev, bounds=bounds, sequence_lengths=sequence_lengths, block_tables=block_tables, query_lens=query_lens,
-                 selected_blocks=selected_blocks, selected_counts=selected_counts, workspace=workspace)
+    dev, index = query.device, query.get_device()
+    _check_devices(index, dev, dict(
+        bounds=bounds, sequence_lengths=sequence_lengths, block_tables=block_tables, query_lens=query_lens, selected_blocks=selected_blocks,
+        selected_counts=selected_counts, workspace=workspace))
     _check_block_size(block_size)
-    _check_sequences(a, sequence_lengths, block_tables, max_sequence_length)
-    _check_bounds(a, bounds)
-    a.num_blocks, a.num_kv_heads, a.block_size = bounds.shape[0], bounds.shape[1], block_size
-    if a.num_blocks < 1 or a.num_kv_heads < 1:
+    num_seqs, width, st_bt = _check_sequences(sequence_lengths, block_tables)
+    st_bb, st_bh = _check_bounds(bounds)
+    blocks, heads, _, head_size = bounds.shape
+    if blocks < 1 or heads < 1:
         raise ValueError(f"bounds shape {tuple(bounds.shape)} is empty")
-    _check_query(a, query, query_sequence_length, a.num_kv_heads, query_lens)
-    if bounds.shape[3] != a.head_size:
-        raise ValueError(f"query has head size {a.head_size}, bounds {bounds.shape[3]}")
-    need_recent = 1 + (a.q_len - 1 + block_size - 1) // block_size
+    q_len, longest, k, first = int(query_sequence_length), max(0, int(max_sequence_length)), int(num_selected), int(first_blocks)
+    group, q_head_size, st_qs, st_qh = _check_query(query, q_len, heads, num_seqs, query_lens)
+    if q_head_size != head_size:
+        raise ValueError(f"query has head size {q_head_size}, bounds {head_size}")
+    need_recent = 1 + (q_len - 1 + block_size - 1) // block_size
     recent = need_recent if recent_blocks is None else int(recent_blocks)
     if recent < need_recent:
-        raise ValueError(f"recent_blocks must be at least {need_recent}: the {a.q_len} new tokens can lie in so many blocks")
-    if int(num_selected) < 1 or int(first_blocks) < 0 or int(first_blocks) + recent > int(num_selected):
+        raise ValueError(f"recent_blocks must be at least {need_recent}: the {q_len} new tokens can lie in so many blocks")
+    if k < 1 or first < 0 or first + recent > k:
         raise ValueError(f"num_selected == {num_selected} does not hold first_blocks + recent_blocks == {first_blocks} + {recent}")
-    if int(num_selected) * block_size > 1 << 30:
+    if k * block_size > 1 << 30:
         raise ValueError(f"num_selected == {num_selected} blocks of {block_size} tokens are too many")
-    a.num_selected, a.first_blocks, a.recent_blocks = int(num_selected), int(first_blocks), recent
     if not query.is_cuda:
         raise ValueError("select_blocks runs on the GPU only (there is no CPU path); got a CPU tensor")
-    shape = (a.num_seqs, a.num_kv_heads)
     if selected_blocks is None:
-        selected_blocks = torch.empty(shape + (a.num_selected,), dtype=torch.int32, device=dev)
-    elif selected_blocks.dtype != torch.int32 or tuple(selected_blocks.shape) != shape + (a.num_selected,) or \
-            (a.num_selected > 1 and selected_blocks.stride(2) != 1):
-        raise ValueError(f"selected_blocks must be int32 {shape + (a.num_selected,)}, contiguous in its last dimension")
+        selected_blocks = torch.empty((num_seqs, heads, k), dtype=torch.int32, device=dev)
+    elif selected_blocks.dtype is not torch.int32 or selected_blocks.shape != (num_seqs, heads, k) or (k > 1 and selected_blocks.stride(2) != 1):
+        raise ValueError(f"selected_blocks must be int32 {(num_seqs, heads, k)}, contiguous in its last dimension")
     if selected_counts is None:
-        selected_counts = torch.empty(shape, dtype=torch.int32, device=dev)
-    elif selected_counts.dtype != torch.int32 or tuple(selected_counts.shape) != shape or \
-            (shape[1] > 1 and selected_counts.stride(1) != 1):
-        raise ValueError(f"selected_counts must be int32 {shape}, dense over the heads")
-    if a.num_seqs:
-        a.selected_blocks, a.selected_counts = selected_blocks.data_ptr(), selected_counts.data_ptr()
-        a.stride_sel_s, a.stride_sel_h = selected_blocks.stride(0), selected_blocks.stride(1)
-        a.stride_cnt_s = selected_counts.stride(0)
-        keep = _give_workspace(a, workspace, _workspace_bytes("pa_select_blocks_workspace_bytes", a), dev)
-        with _on(dev):
-            lib = _cabi.load_library()
-            _cabi.check(lib.pa_select_blocks(C.byref(a), C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "pa_select_blocks")
-        del keep
+        selected_counts = torch.empty((num_seqs, heads), dtype=torch.int32, device=dev)
+    elif selected_counts.dtype is not torch.int32 or selected_counts.shape != (num_seqs, heads) or (heads > 1 and selected_counts.stride(1) != 1):
+        raise ValueError(f"selected_counts must be int32 {(num_seqs, heads)}, dense over the heads")
+    if num_seqs:
+        workspace = _give_workspace(workspace, _select_workspace(num_seqs, heads, group, q_len, head_size, block_size, width, longest), dev)
+        st_ls, st_lh, _ = selected_blocks.stride()
+        args = PaBlockArgs.from_buffer_copy(_PACK.pack(
+            _SIZE, 0,
+            0, query.data_ptr(), 0, 0, 0, 0, sequence_lengths.data_ptr(), block_tables.data_ptr(), _ptr(query_lens), bounds.data_ptr(),
+            selected_blocks.data_ptr(), selected_counts.data_ptr(), 0, workspace.data_ptr(),
+            num_seqs, heads, group, q_len, head_size, block_size, blocks, width, longest, 0, _cabi.PA_QUANT_NONE, 0, k, first, recent, 0,
+            0.0, 0,
+            0, 0, st_qs, st_qh, 0, 0, 0, 0, 0, 0, 0, 0, st_bt, st_bb, st_bh, st_ls, st_lh, selected_counts.stride(0), 0, workspace.numel()))
+        _launch("pa_select_blocks", args, index)
     return selected_blocks, selected_counts

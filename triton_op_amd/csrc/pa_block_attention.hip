@@ -474,6 +474,65 @@ __global__ __launch_bounds__(256) void pa_block_merge_kernel(const PaBlockArgs a
   }
 }
 
+// The same for a few stretches: a wave per row, no barriers.
+constexpr int kFewParts = 16;
+template <int D>
+__global__ __launch_bounds__(256) void pa_block_merge_few_kernel(const PaBlockArgs a, const BlockCut cut) {
+  constexpr int LANES = D / 4, GROUPS = 64 / LANES;
+  const int lane = threadIdx.x & 63;
+  const int Ge = a.q_len * a.group_size;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= (int64_t)a.num_seqs * a.num_kv_heads * Ge) return;
+  const int row = (int)(r % Ge), bh = (int)(r / Ge);
+  const int h = bh % a.num_kv_heads, b = bh / a.num_kv_heads;
+  int ctx = sload_i32(a.context_lens + b);
+  ctx = ctx < 0 ? 0 : (ctx > cut.axis ? cut.axis : ctx);
+  int qb = a.q_lens ? sload_i32(a.q_lens + b) : a.q_len;
+  qb = qb > a.q_len ? a.q_len : qb;
+  const int n = row < qb * a.group_size ? (virtual_tokens(a, b, h, ctx) + cut.part - 1) / cut.part : 0;
+  const int64_t slot0 = (int64_t)bh * cut.parts * Ge + row;
+  const float* po = (const float*)a.workspace + slot0 * D;
+  const float* pm = (const float*)a.workspace + (int64_t)a.num_seqs * a.num_kv_heads * cut.parts * Ge * D + slot0 * 2;
+  // lane p < n holds stretch p's maximum and sum
+  const f32x2 ml = lane < n ? *reinterpret_cast<const f32x2*>(pm + (int64_t)lane * Ge * 2) : f32x2{-INFINITY, 0.f};
+  const int g = lane / LANES, c = lane % LANES;
+  f32x4 v[kFewParts / GROUPS];
+#pragma unroll
+  for (int i = 0; i < kFewParts / GROUPS; ++i) {
+    const int p = i * GROUPS + g;
+    v[i] = p < n ? *reinterpret_cast<const f32x4*>(po + (int64_t)p * Ge * D + 4 * c) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float M = ml[0];
+#pragma unroll
+  for (int o = 1; o < kFewParts; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+  M = __shfl(M, 0);
+  const float f = fast_exp2(ml[0] - (M == -INFINITY ? 0.f : M));
+  float L = lane < n ? f * ml[1] : 0.f;
+#pragma unroll
+  for (int o = 1; o < kFewParts; o <<= 1) L += __shfl_xor(L, o);
+  L = __shfl(L, 0);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kFewParts / GROUPS; ++i) {
+    const float w = __shfl(f, i * GROUPS + g);
+    if (i * GROUPS + g < n) o += v[i] * w;
+  }
+#pragma unroll
+  for (int d = LANES; d < 64; d <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d);
+  }
+  if (g == 0) {
+    const bool ok = L != 0.f;
+    const float inv = ok ? 1.f / L : 0.f;
+    u32x2 w;
+    w[0] = ok ? pack_bf16x2(o[0] * inv, o[1] * inv) : 0u;
+    w[1] = ok ? pack_bf16x2(o[2] * inv, o[3] * inv) : 0u;
+    *reinterpret_cast<u32x2*>((__bf16*)a.output + (int64_t)b * a.stride_out_s + (int64_t)(h * Ge + row) * a.stride_out_h + 4 * c) = w;
+    if (a.lse && c == 0) a.lse[(int64_t)b * a.stride_lse_s + h * Ge + row] = ok ? (M + fast_log2(L)) * (1.f / kLog2e) : -INFINITY;
+  }
+}
+
 int check_attention(const PaBlockArgs* a) {
   if (int rc = check_block_sizes(a)) return rc;
   if (int rc = check_block_rows(a)) return rc;
@@ -562,6 +621,12 @@ int pa_block_attention(const PaBlockArgs* a, void* hip_stream) {
   else
     rc = launch_scale<256, 1>(*a, c, grid, s);
   if (rc || c.parts == 1) return rc;
+  if (c.parts <= kFewParts) {
+    const dim3 few((unsigned)((rows + 3) / 4));
+    return a->head_size == 64    ? pa_launch(pa_block_merge_few_kernel<64>, few, dim3(256), 0, s, *a, c)
+           : a->head_size == 128 ? pa_launch(pa_block_merge_few_kernel<128>, few, dim3(256), 0, s, *a, c)
+                                 : pa_launch(pa_block_merge_few_kernel<256>, few, dim3(256), 0, s, *a, c);
+  }
   const dim3 mgrid((unsigned)rows);
   return a->head_size == 64    ? pa_launch(pa_block_merge_kernel<64>, mgrid, dim3(256), 0, s, *a, c)
          : a->head_size == 128 ? pa_launch(pa_block_merge_kernel<128>, mgrid, dim3(256), 0, s, *a, c)

@@ -63,8 +63,37 @@ struct BoundSlot<kBoundsFp8Token> : BoundSlot32 {};
 template <>
 struct BoundSlot<kBoundsBf16> : BoundSlot32 {};
 
+// lane exchanges inside 16 lanes (DPP).  The pairs of a step need only differ in the bit that picks the half kept and, with the
+// steps before, reach all lanes: 15 - i, then 7 - i, then the neighbour, then the next pair.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kDppSwap1 = 0xB1, kDppSwap2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
+
+// one exchange: the lane keeps the upper or the lower half of its first 2 n slots
+template <int CTRL, int N, typename Slot>
+__device__ __forceinline__ void halve(Slot* slot, bool upper) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t keep = upper ? slot[N + i].bits() : slot[i].bits(), send = upper ? slot[i].bits() : slot[N + i].bits();
+    Slot s;
+    s.take(keep);
+    s.take(dpp_u32<CTRL>(send));
+    slot[i] = s;
+  }
+}
+
 // SPLIT: the four waves of a workgroup share one (sequence, block, kv head) and meet in LDS (blocks of 64 tokens and more);
-// otherwise each has its own.
+// otherwise a wave has kBoundsHeads kv heads of a (sequence, block) and asks for all of their keys before it looks at any:
+// a wave with 2 KiB to read spends its time waiting for the context length, the table and the keys in turn.
+constexpr int kBoundsHeads = 4;
+// kv heads of a wave: fewer where a lane has more loads of a head in flight
+template <int D, int KIND>
+constexpr int bounds_heads() {
+  return 16 / (64 / (D / (KIND == kBoundsBf16 ? 8 : 16))) > 2 ? kBoundsHeads / 2 : kBoundsHeads;
+}
+
 template <int D, int KIND, bool SPLIT>
 __global__ __launch_bounds__(256) void pa_block_bounds_kernel(const PaBlockArgs a, const int axis, const int visits, const unsigned items) {
   typedef BoundSlot<KIND> Slot;
@@ -74,13 +103,15 @@ __global__ __launch_bounds__(256) void pa_block_bounds_kernel(const PaBlockArgs 
   constexpr int HALF = X / Slot::kDims;     // slots of -lo, and as many of hi
   constexpr int KEEP = 2 * HALF / LPC;      // slots a lane is left with
   constexpr int U = 16 / LPC < 4 ? 16 / LPC : 4;  // loads in flight (a 16-token block has 16 / LPC for a lane)
+  constexpr int HEADS = SPLIT ? 1 : bounds_heads<D, KIND>();
   static_assert(KEEP >= 1, "a lane is left with something");
   __shared__ uint32_t meet[SPLIT ? 3 : 1][SPLIT ? KEEP : 1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned item = SPLIT ? blockIdx.x : blockIdx.x * 4 + wave;
   if (item >= items) return;
-  const int h = (int)(item % (unsigned)a.num_kv_heads);
-  const unsigned visit = item / (unsigned)a.num_kv_heads;
+  const unsigned head_groups = ((unsigned)a.num_kv_heads + HEADS - 1) / HEADS;
+  const int h0 = (int)(item % head_groups) * HEADS;
+  const unsigned visit = item / head_groups;
   const int b = (int)(visit / (unsigned)visits);
   const int bs = a.block_size;
   int ctx = sload_i32(a.context_lens + b);
@@ -91,100 +122,129 @@ __global__ __launch_bounds__(256) void pa_block_bounds_kernel(const PaBlockArgs 
   const int page = sload_i32(a.block_tables + (int64_t)b * a.stride_bt_s + at);
   if ((unsigned)page >= (unsigned)a.num_blocks) return;
   const int live = ctx - at * bs < bs ? ctx - at * bs : bs;
-  const char* kp = (const char*)a.key_cache + ((int64_t)page * a.stride_k_b + (int64_t)h * a.stride_k_h + (int64_t)(lane / LPC) * a.stride_k_c) * (FP8 ? 1 : 2);
-  const int64_t so = (int64_t)page * a.stride_kvscale_b + (int64_t)h * a.stride_kvscale_h;
-  float scale = 1.f;
-  if (a.kv_quant_mode == PA_QUANT_PER_TENSOR) scale = sload_f32(a.key_scale);
-  if (a.kv_quant_mode == PA_QUANT_PER_BLOCK) scale = sload_f32(a.key_scale + so);
+  const int heads = min(HEADS, a.num_kv_heads - h0);
+  const char* kp = (const char*)a.key_cache + ((int64_t)page * a.stride_k_b + (int64_t)h0 * a.stride_k_h + (int64_t)(lane / LPC) * a.stride_k_c) * (FP8 ? 1 : 2);
+  const int64_t kh = a.stride_k_h * (FP8 ? 1 : 2);
+  const int64_t so = (int64_t)page * a.stride_kvscale_b + (int64_t)h0 * a.stride_kvscale_h;
 
-  Slot slot[2 * HALF];  // [-lo, hi]
+  Slot slots[HEADS][2 * HALF];  // [-lo, hi]
   constexpr int kTurn = LPC * U * (SPLIT ? 4 : 1);
   for (int t0 = (SPLIT ? wave * LPC * U : 0) + lane % LPC; t0 - lane % LPC < live; t0 += kTurn) {
-    u32x4 w[U];
-    float ts[U];
+    u32x4 w[HEADS][U];
+    float ts[HEADS][U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = t0 + u * LPC < live ? t0 + u * LPC : live - 1;
-      w[u] = load16_stream(kp + t * 16);
-      if constexpr (KIND == kBoundsFp8Token) ts[u] = a.key_scale[so + t];
+    for (int g = 0; g < HEADS; ++g) {
+      const int64_t gh = g < heads ? g : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * LPC < live ? t0 + u * LPC : live - 1;
+        w[g][u] = load16_stream(kp + gh * kh + t * 16);
+        if constexpr (KIND == kBoundsFp8Token) ts[g][u] = a.key_scale[so + gh * a.stride_kvscale_h + t];
+      }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int g = 0; g < HEADS; ++g) {
+      Slot* slot = slots[g];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (KIND == kBoundsFp8) {
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t p = fp8x2_to_f16x2(w[u][i], e);
-            slot[2 * i + e].take(p ^ 0x80008000u);
-            slot[HALF + 2 * i + e].take(p);
-          }
-        } else if constexpr (KIND == kBoundsFp8Token) {
-          const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 0) * ts[u], __builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 1) * ts[u],
-                              __builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 2) * ts[u], __builtin_amdgcn_cvt_f32_fp8((int)w[u][i], 3) * ts[u]};
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t word = w[g][u][i];
+          if constexpr (KIND == kBoundsFp8) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            slot[4 * i + e].take(__float_as_uint(-x[e]));
-            slot[HALF + 4 * i + e].take(__float_as_uint(x[e]));
-          }
-        } else {
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t p = fp8x2_to_f16x2(word, e);
+              slot[2 * i + e].take(p ^ 0x80008000u);
+              slot[HALF + 2 * i + e].take(p);
+            }
+          } else if constexpr (KIND == kBoundsFp8Token) {
+            const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)word, 0) * ts[g][u], __builtin_amdgcn_cvt_f32_fp8((int)word, 1) * ts[g][u],
+                                __builtin_amdgcn_cvt_f32_fp8((int)word, 2) * ts[g][u], __builtin_amdgcn_cvt_f32_fp8((int)word, 3) * ts[g][u]};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t x = e ? w[u][i] & 0xffff0000u : w[u][i] << 16;
-            slot[2 * i + e].take(x ^ 0x80000000u);
-            slot[HALF + 2 * i + e].take(x);
+            for (int e = 0; e < 4; ++e) {
+              slot[4 * i + e].take(__float_as_uint(-x[e]));
+              slot[HALF + 4 * i + e].take(__float_as_uint(x[e]));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t x = e ? word & 0xffff0000u : word << 16;
+              slot[2 * i + e].take(x ^ 0x80000000u);
+              slot[HALF + 2 * i + e].take(x);
+            }
           }
         }
       }
     }
   }
-  // ---- the lanes of a chunk row: step k pairs lanes 2^k apart, the lane with bit k set keeps the upper half --------------------
 #pragma unroll
-  for (int k = 0, n = HALF; (1 << k) < LPC; ++k, n /= 2) {
-    const bool upper = (lane >> k) & 1;
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const uint32_t keep = upper ? slot[n + i].bits() : slot[i].bits(), send = upper ? slot[i].bits() : slot[n + i].bits();
-      Slot s;
-      s.take(keep);
-      s.take((uint32_t)__shfl_xor((int)send, 1 << k));
-      slot[i] = s;
+  for (int g = 0; g < HEADS; ++g) {
+    if (g >= heads) break;
+    Slot* slot = slots[g];
+    // the lanes of a chunk row; `base` is where the slots that are left were
+    int base = 0;
+    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+    if constexpr (LPC == 16) {
+      halve<kDppMirror, HALF>(slot, b3);
+      halve<kDppHalfMirror, HALF / 2>(slot, b2);
+      halve<kDppSwap1, HALF / 4>(slot, b0);
+      halve<kDppSwap2, HALF / 8>(slot, b1);
+      base = b3 * HALF + b2 * (HALF / 2) + b0 * (HALF / 4) + b1 * (HALF / 8);
+    } else if constexpr (LPC == 8) {
+      halve<kDppHalfMirror, HALF>(slot, b2);
+      halve<kDppSwap1, HALF / 2>(slot, b0);
+      halve<kDppSwap2, HALF / 4>(slot, b1);
+      base = b2 * HALF + b0 * (HALF / 2) + b1 * (HALF / 4);
+    } else if constexpr (LPC == 4) {
+      halve<kDppSwap1, HALF>(slot, b0);
+      halve<kDppSwap2, HALF / 2>(slot, b1);
+      base = b0 * HALF + b1 * (HALF / 2);
+    } else {
+      static_assert(LPC == 2 || LPC == 4 || LPC == 8 || LPC == 16, "lanes of a chunk row");
+      halve<kDppSwap1, HALF>(slot, b0);
+      base = b0 * HALF;
     }
-  }
-  if constexpr (SPLIT) {
-    if (wave > 0) {
+    if constexpr (SPLIT) {
+      if (wave > 0) {
 #pragma unroll
-      for (int i = 0; i < KEEP; ++i) meet[wave - 1][i][lane] = slot[i].bits();
+        for (int i = 0; i < KEEP; ++i) meet[wave - 1][i][lane] = slot[i].bits();
+      }
+      __syncthreads();
+      if (wave > 0) return;
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i) {
+#pragma unroll
+        for (int o = 0; o < 3; ++o) slot[i].take(meet[o][i][lane]);
+      }
     }
-    __syncthreads();
-    if (wave > 0) return;
+    float scale = 1.f;
+    if (a.kv_quant_mode == PA_QUANT_PER_TENSOR) scale = sload_f32(a.key_scale);
+    if (a.kv_quant_mode == PA_QUANT_PER_BLOCK) scale = sload_f32(a.key_scale + so + g * a.stride_kvscale_h);
+    const bool is_hi = base >= HALF;
+    const float sign = is_hi ? scale : -scale;
+    // (a negative scale turns the smallest code into the largest key)
+    __bf16* out = (__bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)(h0 + g) * a.stride_bounds_h + (is_hi != (scale < 0.f) ? D : 0) +
+                  lane / LPC * X + (is_hi ? base - HALF : base) * Slot::kDims;
+    constexpr int N = KEEP * Slot::kDims;  // consecutive head dims
+    uint32_t bits[N];
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
+    for (int i = 0; i < N; ++i) bits[i] = __builtin_bit_cast(uint16_t, (__bf16)(slot[i / Slot::kDims].dim(i % Slot::kDims) * sign));
+    if constexpr (N == 1) {
+      *reinterpret_cast<uint16_t*>(out) = (uint16_t)bits[0];
+    } else {
 #pragma unroll
-      for (int o = 0; o < 3; ++o) slot[i].take(meet[o][i][lane]);
+      for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(out + i) = bits[i] | (bits[i + 1] << 16);
     }
-  }
-  // the slots the lane is left with: KEEP of them from `base` on, all of one bound
-  int base = 0;
-#pragma unroll
-  for (int k = 0; (1 << k) < LPC; ++k) base += ((lane >> k) & 1) * (HALF >> k);
-  const bool is_hi = base >= HALF;
-  const float sign = is_hi ? scale : -scale;
-  // (a negative scale turns the smallest code into the largest key)
-  __bf16* out = (__bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)h * a.stride_bounds_h + (is_hi != (scale < 0.f) ? D : 0) +
-                lane / LPC * X + (is_hi ? base - HALF : base) * Slot::kDims;
-#pragma unroll
-  for (int i = 0; i < KEEP; ++i) {
-#pragma unroll
-    for (int e = 0; e < Slot::kDims; ++e) out[i * Slot::kDims + e] = (__bf16)(slot[i].dim(e) * sign);
   }
 }
 
 template <int D, int KIND>
 int launch_bounds(const PaBlockArgs& a, int axis, int visits, hipStream_t s) {
-  const int64_t items = (int64_t)a.num_seqs * visits * a.num_kv_heads;
-  if (items > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
-  if (a.block_size > 16) return pa_launch(pa_block_bounds_kernel<D, KIND, true>, dim3((unsigned)items), dim3(256), 0, s, a, axis, visits, (unsigned)items);
+  const int64_t most = (int64_t)a.num_seqs * visits * a.num_kv_heads;
+  if (most > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
+  if (a.block_size > 16) return pa_launch(pa_block_bounds_kernel<D, KIND, true>, dim3((unsigned)most), dim3(256), 0, s, a, axis, visits, (unsigned)most);
+  const int heads = bounds_heads<D, KIND>();
+  const int64_t items = (int64_t)a.num_seqs * visits * ((a.num_kv_heads + heads - 1) / heads);
   return pa_launch(pa_block_bounds_kernel<D, KIND, false>, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, a, axis, visits, (unsigned)items);
 }
 
@@ -209,13 +269,12 @@ struct BlockScore {
   float s, e;
 };
 
-// lane exchanges inside a row of 16 lanes (DPP): the maximum over the row
-template <int CTRL>
-__device__ __forceinline__ float dpp_max(float v) {
-  return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true)));
-}
+// the maximum over a row of 16 lanes
 __device__ __forceinline__ float row16_max(float v) {
-  return dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));  // quad_perm swaps, half mirror, mirror
+  v = fmaxf(v, __uint_as_float(dpp_u32<kDppSwap1>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(dpp_u32<kDppSwap2>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(v))));
+  return fmaxf(v, __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(v))));
 }
 
 constexpr int kScoreWaves = 4;

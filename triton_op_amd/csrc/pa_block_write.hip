@@ -66,8 +66,11 @@ __device__ __forceinline__ u32x4 load_row8(const uint16_t* p) {
   }
 }
 
-// eight codes of x / s for a power of two s = 1 / inv (the product is then the quotient), or any s
-__device__ __forceinline__ u32x2 quantize_row8(u32x4 x, float s, float inv, bool pow2) {
+// Eight codes of x / s, given 1 / s in 64 bits.  For a power of two s the 32-bit product is the quotient.  For any other s
+// the 64-bit product, rounded to 32 bits, is the correctly rounded 32-bit quotient: x has 8 significant bits and s 24, so x / s
+// is never closer than 2^-49 to a midpoint of 32-bit numbers (that midpoint times s has 25 significant bits or more, x has 8),
+// and the product is off by 2^-51 at most.
+__device__ __forceinline__ u32x2 quantize_row8(u32x4 x, double inv, bool pow2) {
   u32x2 out;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
@@ -75,8 +78,15 @@ __device__ __forceinline__ u32x2 quantize_row8(u32x4 x, float s, float inv, bool
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t p = x[2 * w + (e >> 1)];
-      const float f = __uint_as_float(e & 1 ? p & 0xffff0000u : p << 16);
-      v[e] = pow2 ? f * inv : __fdiv_rn(f, s);
+      v[e] = __uint_as_float(e & 1 ? p & 0xffff0000u : p << 16);
+    }
+    if (pow2) {
+      const float r = (float)inv;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= r;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (float)((double)v[e] * inv);
     }
     out[w] = to_codes(v[0], v[1], v[2], v[3]);
   }
@@ -162,7 +172,7 @@ __device__ __forceinline__ void write_block_head(const PaKvWriteArgs& a, const l
   const float ratio_k = grow_k ? __fdiv_rn(old_k, new_k) : 1.f, ratio_v = grow_v ? __fdiv_rn(old_v, new_v) : 1.f;
   auto is_pow2 = [](float s) { return (__float_as_uint(s) & 0x7fffffu) == 0 && s >= 0x1p-126f && s <= 0x1p126f; };
   const bool pow2_k = is_pow2(new_k), pow2_v = is_pow2(new_v);
-  const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
+  const double inv_k = 1.0 / (double)new_k, inv_v = 1.0 / (double)new_v;
   if (lane == 0) {
     a.key_scale[so] = new_k;
     a.value_scale[so] = new_v;
@@ -182,7 +192,7 @@ __device__ __forceinline__ void write_block_head(const PaKvWriteArgs& a, const l
     for (int j = 0; j < R; ++j) {
       const int slot = 16 * seg + lane / P + 64 / P * j, c = lane % P;
       if (owner[slot] >= 0)
-        *reinterpret_cast<u32x2*>(kc + ((int64_t)(c >> 1) * bs + slot) * 16 + 8 * (c & 1)) = quantize_row8(kr[j], new_k, inv_k, pow2_k);
+        *reinterpret_cast<u32x2*>(kc + ((int64_t)(c >> 1) * bs + slot) * 16 + 8 * (c & 1)) = quantize_row8(kr[j], inv_k, pow2_k);
     }
     if (grow_k) {
 #pragma unroll
@@ -200,7 +210,7 @@ __device__ __forceinline__ void write_block_head(const PaKvWriteArgs& a, const l
     if (members || grow_v) {
 #pragma unroll
       for (int j = 0; j < R; ++j)
-        *reinterpret_cast<u32x2*>(&turn[lane / P + 64 / P * j][lane % P * 8]) = quantize_row8(vr[j], new_v, inv_v, pow2_v);
+        *reinterpret_cast<u32x2*>(&turn[lane / P + 64 / P * j][lane % P * 8]) = quantize_row8(vr[j], inv_v, pow2_v);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -236,7 +246,8 @@ __device__ __forceinline__ void write_block_head(const PaKvWriteArgs& a, const l
 // grid: (windows of `window` tokens) x (groups of `heads` kv heads).  ALIGNED: the rows can be read 16 bytes at a time.
 template <int D, bool ALIGNED>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_block_scaled_kernel(const PaKvWriteArgs a, const long long num_slots,
-                                                                               const int bs_shift, const int window, const int heads) {
+                                                                               const int bs_shift, const int window, const int turn_bits,
+                                                                               const int heads) {
   __shared__ int owner[kMaxBlockSize];     // per slot of the block: the latest token of the call, -1 without one
   __shared__ unsigned long long segments;  // bit i: 16-slot segment i gets a token
   __shared__ int earlier;
@@ -245,9 +256,15 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_block_scaled_kernel(c
   const int bs = 1 << bs_shift;
   const int num_tokens = (int)a.num_tokens;
   const int head_groups = (a.num_kv_heads + heads - 1) / heads;
+  // Workgroups are handed out in id order, round the XCDs and round the shader engines of each, and one that has to wait for
+  // its engine holds up the next.  In a prompt every fourth window owns a block (16-token blocks): in plain order these
+  // would all be one engine's (measured: 4 times the time).  Bits of the id in reverse order make them neighbours.
+  const unsigned unit = blockIdx.x / (unsigned)head_groups, group = (1u << turn_bits) - 1;
+  const unsigned turned = turn_bits ? __builtin_bitreverse32(unit & group) >> (32 - turn_bits) : 0;
+  const long long t0 = (long long)((unit & ~group) | turned) * window;
+  if (t0 >= num_tokens) return;
   const int h0 = (int)(blockIdx.x % (unsigned)head_groups) * heads;
   const int h1 = h0 + heads < a.num_kv_heads ? h0 + heads : a.num_kv_heads;
-  const long long t0 = (long long)(blockIdx.x / (unsigned)head_groups) * window;
   const int t_end = (int)(t0 + window < num_tokens ? t0 + window : num_tokens);
 
   auto block_of = [&](long long slot) -> long long { return slot < 0 || slot >= num_slots ? -1 : slot >> bs_shift; };
@@ -268,15 +285,24 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_block_scaled_kernel(c
       segments = 0;
     }
     __syncthreads();
-#pragma unroll 8
-    for (int i = tid; i < num_tokens; i += kThreads) {
-      const long long slot = a.slot_mapping[i];
-      if (block_of(slot) != block) continue;
-      if (i < t) {
-        earlier = 1;
-      } else {
-        atomicMax(&owner[slot & (bs - 1)], i);
-        atomicOr(&segments, 1ull << ((slot & (bs - 1)) >> 4));
+    // (eight slots of a thread are asked for at a time: one by one this would be a chain of L2 latencies)
+    for (int i0 = tid; i0 < num_tokens; i0 += 8 * kThreads) {
+      long long slot[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * kThreads;
+        slot[u] = i < num_tokens ? a.slot_mapping[i] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (block_of(slot[u]) != block) continue;
+        const int i = i0 + u * kThreads, off = (int)(slot[u] & (bs - 1));
+        if (i < t) {
+          earlier = 1;
+        } else {
+          atomicMax(&owner[off], i);
+          atomicOr(&segments, 1ull << (off >> 4));
+        }
       }
     }
     __syncthreads();
@@ -303,18 +329,22 @@ extern "C" int pa_kv_cache_write_block_scaled(const PaKvWriteArgs* a, int64_t nu
   const uintptr_t rows = reinterpret_cast<uintptr_t>(a->key) | reinterpret_cast<uintptr_t>(a->value);
   const bool aligned = (rows & 15) == 0 && a->stride_k_t % 8 == 0 && a->stride_k_h % 8 == 0 && a->stride_v_t % 8 == 0 && a->stride_v_h % 8 == 0;
   // A few tokens (decode): one workgroup per (token, four kv heads).  Many (prompts): most tokens own no block, so a
-  // workgroup looks at 16 of them, and walks all kv heads so that the slot mapping is read once per block.
+  // workgroup looks at four of them, and walks all kv heads so that the slot mapping is read once per block (8192 tokens, 8
+  // heads: 28 us with windows of 16, where one workgroup in a prompt has two blocks, 23 with 4).
   const bool many = a->num_tokens > 1024;
-  const int window = many ? 16 : 1, heads = many ? a->num_kv_heads : kThreads / 64;
-  const int64_t grid = ((a->num_tokens + window - 1) / window) * ((a->num_kv_heads + heads - 1) / heads);
+  const int window = many ? 4 : 1, heads = many ? a->num_kv_heads : kThreads / 64;
+  const int64_t windows = (a->num_tokens + window - 1) / window;
+  int turn_bits = 0;
+  while (turn_bits < 10 && (1 << turn_bits) < windows) ++turn_bits;
+  const int64_t grid = ((windows + (1 << turn_bits) - 1) >> turn_bits << turn_bits) * ((a->num_kv_heads + heads - 1) / heads);
   if (grid > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
   const int shift = __builtin_ctz((unsigned)a->block_size);
   const long long num_slots = num_blocks << shift;
   hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
   const dim3 g((unsigned)grid), b(kThreads);
 #define PA_WRITE(D)                                                                                                               \
-  (aligned ? pa_launch(kv_cache_write_block_scaled_kernel<D, true>, g, b, 0, stream, *a, num_slots, shift, window, heads)         \
-           : pa_launch(kv_cache_write_block_scaled_kernel<D, false>, g, b, 0, stream, *a, num_slots, shift, window, heads))
+  (aligned ? pa_launch(kv_cache_write_block_scaled_kernel<D, true>, g, b, 0, stream, *a, num_slots, shift, window, turn_bits, heads)         \
+           : pa_launch(kv_cache_write_block_scaled_kernel<D, false>, g, b, 0, stream, *a, num_slots, shift, window, turn_bits, heads))
   return a->head_size == 64 ? PA_WRITE(64) : a->head_size == 128 ? PA_WRITE(128) : PA_WRITE(256);
 #undef PA_WRITE
 }

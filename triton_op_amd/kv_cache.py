@@ -9,6 +9,7 @@ and are what the tests compare them with.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -18,9 +19,21 @@ from ._cabi import PaKvWriteArgs
 
 FP8_DTYPE = torch.float8_e4m3fn
 
+# PaKvWriteArgs in one go, in the order of its fields
+_PACK = struct.Struct("<Ii7Qq6i10q")
+assert _PACK.size == C.sizeof(PaKvWriteArgs)
+
+# the handle of torch's current stream without the Stream object around it (1 us of a small call)
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def _stream(dev) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, ...]:
+    """Strides with 0 for a dimension of size 1, whose stride means nothing."""
+    return tuple(st if n > 1 else 0 for n, st in zip(t.shape, t.stride()))
 
 
 def quantize_kv_cache_symmetric(
@@ -97,17 +110,12 @@ def kv_cache_write(
         raise ValueError("cache shapes must be [blocks, Hkv, D/x, bs, x] and [blocks, Hkv, D, bs] "
                          "(or [blocks, Hkv, bs/x, D, x] for the transposed V layout)")
     v_dense = (d * x, x, 1) if v_transposed else (bs, 1)
-    def _dense(t, want):  # the stride of a dimension of size 1 means nothing
-        return all(n == 1 or st == w for n, st, w in zip(t.shape, t.stride(), want))
+    def _dense(t, want):  # the dimensions inside a (block, head); the stride of a dimension of size 1 means nothing
+        return all(n == 1 or st == w for n, st, w in zip(t.shape[2:], t.stride()[2:], want))
 
-    if not _dense(key_cache[0, 0], (bs * x, x, 1)) or not _dense(value_cache[0, 0], v_dense):
+    if not _dense(key_cache, (bs * x, x, 1)) or not _dense(value_cache, v_dense):
         raise ValueError("the cache dimensions inside a (block, head) must be dense")
-    a = PaKvWriteArgs()
-    a.struct_size = C.sizeof(PaKvWriteArgs)
-    a.key, a.value, a.slot_mapping = key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr()
-    a.key_cache, a.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
-    a.num_tokens, a.num_kv_heads, a.head_size, a.block_size = t, h, d, bs
-    a.cache_dtype = _cabi.PA_DTYPE_FP8_E4M3FN if key_cache.dtype == FP8_DTYPE else _cabi.PA_DTYPE_BF16
+    st_sb = st_sh = 0
     mode = _cabi.PA_QUANT_NONE
     if key_scale is not None or value_scale is not None:
         if key_scale is None or value_scale is None or key_scale.shape != value_scale.shape or \
@@ -118,28 +126,31 @@ def kv_cache_write(
         if key_scale.dim() == 0:
             mode = _cabi.PA_QUANT_PER_TENSOR
         elif tuple(key_scale.shape) == (key_cache.shape[0], h, 1, 1) and bs != 1:
-            if key_scale.stride() != value_scale.stride():
+            if _strides(key_scale) != _strides(value_scale):
                 raise ValueError("key_scale and value_scale must have the same strides")
             mode = _cabi.PA_QUANT_PER_BLOCK
-            a.stride_scale_b, a.stride_scale_h = key_scale.stride(0), key_scale.stride(1)
+            st_sb, st_sh = key_scale.stride(0), key_scale.stride(1)
         else:
             if tuple(key_scale.shape) != (key_cache.shape[0], h, bs, 1) or key_scale.stride(2) != 1 or \
                     key_scale.stride() != value_scale.stride():
                 raise ValueError(f"per-token scales must be [blocks, {h}, {bs}, 1], dense over tokens, same strides")
             mode = _cabi.PA_QUANT_PER_TOKEN
-            a.stride_scale_b, a.stride_scale_h = key_scale.stride(0), key_scale.stride(1)
-        a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
-    a.kv_quant_mode = mode
-    a.v_transposed = 1 if v_transposed else 0
-    a.stride_k_t, a.stride_k_h, a.stride_v_t, a.stride_v_h = key.stride(0), key.stride(1), value.stride(0), value.stride(1)
-    a.stride_kc_b, a.stride_kc_h = key_cache.stride(0), key_cache.stride(1)
-    a.stride_vc_b, a.stride_vc_h = value_cache.stride(0), value_cache.stride(1)
+            st_sb, st_sh = key_scale.stride(0), key_scale.stride(1)
+    st_kc, st_vc = key_cache.stride(), value_cache.stride()
+    a = PaKvWriteArgs.from_buffer_copy(_PACK.pack(
+        _PACK.size, 0,
+        key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+        0 if key_scale is None else key_scale.data_ptr(), 0 if value_scale is None else value_scale.data_ptr(),
+        t, h, d, bs, _cabi.PA_DTYPE_FP8_E4M3FN if key_cache.dtype == FP8_DTYPE else _cabi.PA_DTYPE_BF16, mode, v_transposed,
+        key.stride(0), key.stride(1), value.stride(0), value.stride(1), st_kc[0], st_kc[1], st_vc[0], st_vc[1], st_sb, st_sh))
     lib = _cabi.load_library()
-    if mode == _cabi.PA_QUANT_PER_BLOCK:
-        if key_cache.shape[0] != value_cache.shape[0]:
-            raise ValueError(f"key_cache has {key_cache.shape[0]} blocks, value_cache {value_cache.shape[0]}")
-        with torch.cuda.device(key.device):
-            _cabi.check(lib.pa_kv_cache_write_block_scaled(C.byref(a), key_cache.shape[0], _stream(key.device)),
-                        "pa_kv_cache_write_block_scaled")
+    if mode != _cabi.PA_QUANT_PER_BLOCK:
+        _cabi.check(lib.pa_kv_cache_write(C.byref(a), _stream(key.device)), "pa_kv_cache_write")
         return
-    _cabi.check(lib.pa_kv_cache_write(C.byref(a), _stream(key.device)), "pa_kv_cache_write")
+    blocks, index = key_cache.shape[0], key.get_device()
+    if blocks != value_cache.shape[0]:
+        raise ValueError(f"key_cache has {blocks} blocks, value_cache {value_cache.shape[0]}")
+    with torch.cuda.device(index):
+        rc = lib.pa_kv_cache_write_block_scaled(C.byref(a), blocks, _current_raw_stream(index))
+    if rc:
+        _cabi.check(rc, "pa_kv_cache_write_block_scaled")
