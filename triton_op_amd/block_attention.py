@@ -153,13 +153,13 @@ def _check_bounds(bounds) -> Tuple[int, int]:
 
 
 @functools.lru_cache(maxsize=4096)
-def _attention_workspace(num_seqs, heads, group, q_len, head_size, bs, width, longest, num_selected) -> int:
+def _attention_workspace(num_seqs, heads, group, q_len, head_size, bs, code, width, longest, num_selected) -> int:
     """pa_block_attention_workspace_bytes, a pure function of these sizes."""
     aligned = 1 << 12  # (an address that passes the library's checks and is not followed)
     a = PaBlockArgs(struct_size=_SIZE, output=aligned, query=aligned, key_cache=aligned, value_cache=aligned, context_lens=aligned,
                     block_tables=aligned, num_seqs=num_seqs, num_kv_heads=heads, group_size=group, q_len=q_len, head_size=head_size,
-                    block_size=bs, num_blocks=1, table_width=width, max_context_len=longest, kv_quant_mode=_cabi.PA_QUANT_NONE,
-                    selected_blocks=aligned if num_selected else None, num_selected=num_selected)
+                    block_size=bs, kv_dtype=code, num_blocks=1, table_width=width, max_context_len=longest,
+                    kv_quant_mode=_cabi.PA_QUANT_NONE, selected_blocks=aligned if num_selected else None, num_selected=num_selected)
     return _workspace_bytes("pa_block_attention_workspace_bytes", a)
 
 
@@ -275,7 +275,7 @@ def plan_block_attention(
     if not output.is_cuda:
         raise ValueError("paged_block_attention runs on the GPU only (there is no CPU path); got a CPU tensor")
     if num_seqs:
-        need = _attention_workspace(num_seqs, heads, group, q_len, head_size, bs, width, longest, num_selected)
+        need = _attention_workspace(num_seqs, heads, group, q_len, head_size, bs, code, width, longest, num_selected)
         workspace = _give_workspace(workspace, need, dev)
     args = PaBlockArgs.from_buffer_copy(_PACK.pack(
         _SIZE, 0,

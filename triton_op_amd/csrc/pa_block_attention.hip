@@ -49,18 +49,28 @@ __device__ __forceinline__ int virtual_tokens(const PaBlockArgs& a, int b, int h
   return ctx > 0 ? n * a.block_size : 0;
 }
 
-template <int D, bool FP8, int SCALE, int NT, bool STREAM>
-__global__ __launch_bounds__(64 * kBlockWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// STEP: tokens a wave takes at a time, 64 or 32 (half the registers in flight: head size 256, 16-bit caches, four tiles).  A lane
+// group holds the STEP / 4 consecutive tokens kg * STEP / 4 .. of it, the whole or the half of a 16-token piece.
+// Q_LDS: the query operands wait in LDS (the same for the four waves) and not in registers.
+// OCC: waves per SIMD that the registers are cut for.
+template <int D, bool FP8, int SCALE, int NT, int STEP, int OCC, bool Q_LDS, bool STREAM>
+__global__ __launch_bounds__(64 * kBlockWaves) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
   constexpr int ESZ = FP8 ? 1 : 2;
   constexpr int X = FP8 ? 16 : 8;            // cache elements per 16 bytes
   constexpr int KL = D / (4 * X);            // 16-byte K loads per lane and tile
-  constexpr int VL = FP8 ? 1 : 2;            // 16-byte V loads per lane and 16 head dims
   constexpr int KM = D / 32;                 // MFMAs per tile of S
   constexpr int DB = D / 16;                 // 16-dim rows of O
+  constexpr int NP = STEP / 16;              // pieces of a step, and tiles of S
+  constexpr int TPL = STEP / 4;              // tokens of a lane
+  constexpr int U = TPL / 8;                 // MFMAs per 16 dims of O and P term
+  constexpr int VW = TPL * ESZ / 4;          // V words per lane and 16 dims
   constexpr int OROW = D + 4;                // floats per row of the merge buffer (padded: rows on different banks)
+  static_assert(STEP == 64 || STEP == 32, "a lane has a whole piece or half of one");
   __shared__ __attribute__((aligned(16))) float o_lds[kBlockWaves][16][OROW];
   __shared__ float m_lds[kBlockWaves][16], l_lds[kBlockWaves][16];
+  u32x4* const q_lds = reinterpret_cast<u32x4*>(&o_lds[0][0][0]);  // (the query operands, until the waves merge)
+  static_assert(!Q_LDS || NT * KM * 64 * 16 <= (int)sizeof(o_lds), "the query operands fit where the waves merge");
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -97,26 +107,7 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
   qb = qb < 0 ? 0 : (qb > a.q_len ? a.q_len : qb);
   const int rows_valid = qb * G;
 
-  // ---- this lane's query rows ------------------------------------------------------------------------------------------
-  bf16x8 q[NT][KM];
-  int limit[NT];  // keys the row sees (causal over the new tokens)
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int row = row0 + 16 * n + li;
-    const bool ok = row < rows_valid;
-    limit[n] = ok ? ctx - (qb - 1 - row / G) : 0;
-    const __bf16* qp = (const __bf16*)a.query + (int64_t)b * a.stride_q_s + (int64_t)(h * Ge + (ok ? row : 0)) * a.stride_q_h;
-#pragma unroll
-    for (int c = 0; c < KM; ++c) {
-      // FP8: MFMA c = 2 g + m takes head dims 64 g + 16 kg + 8 m .. + 7 (half of the lane's 16-byte piece); bf16: 32 c + 8 kg .. + 7
-      const int d = FP8 ? 64 * (c >> 1) + 16 * kg + 8 * (c & 1) : 32 * c + 8 * kg;
-      Bf16x8Bits r;
-      r.u = load16(qp + d);
-      if (!ok) r.u = u32x4{0, 0, 0, 0};
-      q[n][c] = r.v;
-    }
-  }
-  const int limit_all = ctx - (a.q_len - 1);  // keys that every row sees, at least
+  // logits in the log2 domain: k_factor * (q . k), with the factor's sign moved into q (a maximum is then one of q . k)
   float k_factor = a.softmax_scale * kLog2e, v_factor = 1.f;
   if constexpr (SCALE == kScaleOne) {
     if (a.kv_quant_mode == PA_QUANT_PER_TENSOR) {
@@ -124,6 +115,42 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
       v_factor = sload_f32(a.value_scale);
     }
   }
+  const uint32_t flip = k_factor < 0.f ? 0x80008000u : 0u;
+  k_factor = fabsf(k_factor);
+
+  // ---- the query rows: FP8, MFMA c = 2 g + m takes head dims 64 g + 16 kg + 8 m .. + 7 (half of the lane's 16-byte
+  // piece of K); bf16, 32 c + 8 kg .. + 7 ---------------------------------------------------------------------------------
+  bf16x8 q[Q_LDS ? 1 : NT][Q_LDS ? 1 : KM];
+  auto query_operand = [&](int n, int c) {
+    const int row = row0 + 16 * n + li;
+    const int d = FP8 ? 64 * (c >> 1) + 16 * kg + 8 * (c & 1) : 32 * c + 8 * kg;
+    u32x4 r = {0, 0, 0, 0};
+    if (row < rows_valid) r = load16((const __bf16*)a.query + (int64_t)b * a.stride_q_s + (int64_t)(h * Ge + row) * a.stride_q_h + d) ^ flip;
+    return r;
+  };
+  if constexpr (Q_LDS) {
+    for (int i = wave; i < NT * KM; i += kBlockWaves) q_lds[i * 64 + lane] = query_operand(i / KM, i % KM);
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < KM; ++c) q[n][c] = Bf16x8Bits{.u = query_operand(n, c)}.v;
+    }
+  }
+  auto q_of = [&](int n, int c) {
+    if constexpr (Q_LDS)
+      return Bf16x8Bits{.u = q_lds[(n * KM + c) * 64 + lane]}.v;
+    else
+      return q[n][c];
+  };
+  int limit[NT];  // keys the lane's row sees (causal over the new tokens)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = row0 + 16 * n + li;
+    limit[n] = row < rows_valid ? ctx - (qb - 1 - row / G) : 0;
+  }
+  const int limit_all = ctx - (a.q_len - 1);  // keys that every row sees, at least
 
   const int log2_bs = 31 - __builtin_clz(a.block_size);
   const int bs_mask = a.block_size - 1;
@@ -138,13 +165,13 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
   // is not there (behind the stretch, a number outside the sequence, an entry outside the cache) reads block 0 and has a
   // position behind every context.
   struct Pieces {
-    int page[4], off[4], pos[4];
+    int page[NP], off[NP], pos[NP];
   };
   constexpr int kNowhere = 0x7fffff00;
   auto fetch = [&](int tok0) {
     Pieces p;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NP; ++j) {
       const int t = tok0 + 16 * j;
       const bool in = t < wg_end;
       const int idx = in ? t >> log2_bs : 0;
@@ -158,35 +185,53 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
     }
     return p;
   };
-  const int sub = li >> 2;  // the piece this lane's K rows come from; kg is the one its logits and V belong to
-  auto pick = [](const int (&v)[4], int i) { return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3]; };
-  auto load = [](const char* p) {
-    if constexpr (STREAM)
-      return load16_stream(p);
+  // the piece of lane group g, and where in it the group's tokens begin
+  auto pick = [](const int (&v)[NP], int g) {
+    if constexpr (NP == 4)
+      return g == 0 ? v[0] : g == 1 ? v[1] : g == 2 ? v[2] : v[3];
     else
-      return load16(p);
+      return g < 2 ? v[0] : v[1];
   };
+  auto inside = [](int g) { return NP == 4 ? 0 : 8 * (g & 1); };
+  const int sub = li >> 2;  // the lane group whose tokens this lane's K rows are; kg is the one its logits and V are of
 
-  u32x4 kr[4][KL], vr[DB][VL];
-  f32x4 ks[SCALE == kScaleToken ? 4 : 1], vs[SCALE == kScaleToken ? 4 : 1];
+  u32x4 kr[NP][KL];
+  uint32_t vr[DB][VW];
+  f32x4 ks[SCALE == kScaleToken ? NP : 1], vs[SCALE == kScaleToken ? NP : 1];
   float ks1 = 1.f, vs1 = 1.f;
   auto load_k = [&](const Pieces& p) {
-    const char* kt = kbase + (int64_t)pick(p.page, sub) * a.stride_k_b * ESZ + (pick(p.off, sub) + (li & 3)) * 16;
+    const char* kt = kbase + (int64_t)pick(p.page, sub) * a.stride_k_b * ESZ + (pick(p.off, sub) + inside(sub) + (li & 3)) * 16;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NP; ++j) {
 #pragma unroll
-      for (int g = 0; g < KL; ++g) kr[j][g] = load(kt + (int64_t)(4 * g + kg) * a.stride_k_c * ESZ + 64 * j);
+      for (int g = 0; g < KL; ++g) {
+        const char* src = kt + (int64_t)(4 * g + kg) * a.stride_k_c * ESZ + 64 * j;
+        kr[j][g] = STREAM ? load16_stream(src) : load16(src);
+      }
     }
   };
   auto load_v = [&](const Pieces& p) {
-    const int off = pick(p.off, kg);
+    const int off = pick(p.off, kg) + inside(kg);
     const char* vt = vbase + (int64_t)pick(p.page, kg) * a.stride_v_b * ESZ;
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
       const int d = 16 * db + li;
-      const int64_t e = a.v_transposed ? (int64_t)(off / X) * a.stride_v_2 + d * X : (int64_t)d * a.stride_v_2 + off;
-      vr[db][0] = load(vt + e * ESZ);
-      if constexpr (VL == 2) vr[db][1] = load(vt + (e + (a.v_transposed ? a.stride_v_2 : 8)) * ESZ);
+      const int64_t e = a.v_transposed ? (int64_t)(off / X) * a.stride_v_2 + d * X + off % X : (int64_t)d * a.stride_v_2 + off;
+      const char* src = vt + e * ESZ;
+      if constexpr (VW == 2) {
+        const u32x2 w = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(src)) : *reinterpret_cast<const u32x2*>(src);
+        vr[db][0] = w[0];
+        vr[db][1] = w[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VW; i += 4) {
+          // (bf16, 16 tokens: the second eight are the next tile of a transposed cache)
+          const char* s = i == 0 ? src : src + (a.v_transposed ? a.stride_v_2 : 8) * ESZ;
+          const u32x4 w = STREAM ? load16_stream(s) : load16(s);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) vr[db][i + k] = w[k];
+        }
+      }
     }
   };
   auto load_scales = [&](const Pieces& p) {
@@ -195,16 +240,37 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
       ks1 = a.key_scale[so];
       vs1 = a.value_scale[so];
     } else if constexpr (SCALE == kScaleToken) {
-      const int off = pick(p.off, kg);
+      const int off = pick(p.off, kg) + inside(kg);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NP; ++j) {
         ks[j] = *reinterpret_cast<const f32x4*>(a.key_scale + so + off + 4 * j);
         vs[j] = *reinterpret_cast<const f32x4*>(a.value_scale + so + off + 4 * j);
       }
     }
   };
+  // eight tokens (FP8: two words, bf16: four) of a head dim as an MFMA operand, times a power of two (FP8)
+  auto v_operand = [&](int db, int u, float pow2) {
+    if constexpr (FP8) {
+      typedef __attribute__((ext_vector_type(2))) __bf16 pair;
+      union {
+        pair p[4];
+        bf16x8 v;
+      } r;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        r.p[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vr[db][2 * u + i], pow2, false);
+        r.p[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vr[db][2 * u + i], pow2, true);
+      }
+      return r.v;
+    } else {
+      return Bf16x8Bits{.u = u32x4{vr[db][4 * u], vr[db][4 * u + 1], vr[db][4 * u + 2], vr[db][4 * u + 3]}}.v;
+    }
+  };
 
-  float m_run[NT], l_run[NT];  // running maximum (log2 domain) and sum of row li, the same in the row's four lanes
+  // The reference m_run of row li's sums (log2 domain; the same in the row's four lanes) follows the row's maximum only when
+  // that is more than kLag above it: probabilities up to 2^kLag cost no precision, and most steps rescale nothing.
+  constexpr float kLag = 8.f;
+  float m_run[NT], l_run[NT];
   f32x4 acc[NT][DB];           // O^T: head dims 16 db + 4 kg .. + 3 of row li
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -214,8 +280,8 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
     for (int db = 0; db < DB; ++db) acc[n][db] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  constexpr int kStride = kBlockWaves * kStepTokens;
-  int tok0 = wg_start + wave * kStepTokens;
+  constexpr int kStride = kBlockWaves * STEP;
+  int tok0 = wg_start + wave * STEP;
   if (tok0 < wg_end) {
     Pieces now = fetch(tok0);
     load_k(now);
@@ -224,10 +290,12 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
     Pieces next = fetch(tok0 + kStride);
     for (; tok0 < wg_end; tok0 += kStride) {
       const bool more = tok0 + kStride < wg_end;
+      // (the compiler would otherwise read the query operands once, in front of the loop, into registers that are not there)
+      if constexpr (Q_LDS) asm volatile("" ::: "memory");
       // ---- S^T = K Q^T ------------------------------------------------------------------------------------------------
-      f32x4 s[NT][4];
+      f32x4 s[NT][NP];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NP; ++j) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -236,23 +304,23 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
             const bf16x8 k0 = fp8x8_to_bf16x8(kr[j][g][0], kr[j][g][1]), k1 = fp8x8_to_bf16x8(kr[j][g][2], kr[j][g][3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[n][2 * g], s[n][j], 0, 0, 0);
-              s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[n][2 * g + 1], s[n][j], 0, 0, 0);
+              s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q_of(n, 2 * g), s[n][j], 0, 0, 0);
+              s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q_of(n, 2 * g + 1), s[n][j], 0, 0, 0);
             }
           } else {
             Bf16x8Bits k0;
             k0.u = kr[j][g];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0.v, q[n][g], s[n][j], 0, 0, 0);
+            for (int n = 0; n < NT; ++n) s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0.v, q_of(n, g), s[n][j], 0, 0, 0);
           }
         }
       }
       // this step's scales; the registers are about to take the next step's
-      f32x4 ks_now[SCALE == kScaleToken ? 4 : 1], vs_now[SCALE == kScaleToken ? 4 : 1];
+      f32x4 ks_now[SCALE == kScaleToken ? NP : 1], vs_now[SCALE == kScaleToken ? NP : 1];
       float ks1_now = ks1, vs1_now = vs1;
       if constexpr (SCALE == kScaleToken) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NP; ++j) {
           ks_now[j] = ks[j];
           vs_now[j] = vs[j];
         }
@@ -261,43 +329,78 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
         load_k(next);
         load_scales(next);
       }
-      // ---- softmax (s[n][j][r]: token 4 j + r of piece kg) ----------------------------------------------------------------
-      const int pos = pick(now.pos, kg);
-      const bool clean = __all(pos + 16 <= limit_all);
-      const int live = ctx - pos;  // live tokens of the lane's piece (may be <= 0 or >= 16)
+      // ---- softmax (s[n][j][r]: token 4 j + r of the lane's) --------------------------------------------------------------
+      const int pos = pick(now.pos, kg) + inside(kg);
+      const bool clean = __all(pos + TPL <= limit_all);
+      const int live = ctx - pos;  // live tokens of the lane's (may be <= 0 or >= TPL)
       if (!clean) {  // a scale behind the context may be NaN, and 0 * NaN is NaN
         if constexpr (SCALE == kScaleBlock) vs1_now = live > 0 ? vs1_now : 0.f;
         if constexpr (SCALE == kScaleToken) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < NP; ++j) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) vs_now[j][r] = 4 * j + r < live ? vs_now[j][r] : 0.f;
           }
         }
-      }
-      bf16x8 hi[NT][2], lo[NT][2];
+        // bytes behind the context may decode to NaN: those tokens' V is zero
+        if (__any(live < TPL)) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float mx = -INFINITY;
+          for (int db = 0; db < DB; ++db) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = s[n][j][r] * (SCALE == kScaleBlock ? ks1_now * k_factor : k_factor);
-            if constexpr (SCALE == kScaleToken) x *= ks_now[j][r];
-            if (!clean) x = pos + 4 * j + r < limit[n] ? x : -INFINITY;  // (a select: bytes behind the context may be NaN)
-            s[n][j][r] = x;
-            mx = fmaxf(mx, x);
+            for (int w = 0; w < VW; ++w) {
+              const int n = live - w * (4 / ESZ);  // live tokens from this word on
+              vr[db][w] &= n >= 4 / ESZ ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * ESZ * n)) - 1u);
+            }
           }
         }
-        mx = quad_row_max(mx);
-        const float m_new = fmaxf(m_run[n], mx);
-        const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = fast_exp2(m_run[n] - m_safe);  // exp2(-inf) = 0 while the row has seen no key
-        m_run[n] = m_new;
+      }
+      // V's scale is 2^e v_rest with v_rest in [1, 2): the power is applied when the codes are converted, v_rest as a summand of
+      // the probabilities' exponents, which the lane's sum is rid of again (both are exactly nothing for a power of two)
+      float v_pow2 = 1.f, v_log2 = 0.f, v_inv = 1.f;
+      if constexpr (SCALE == kScaleBlock) {
+        const uint32_t bits = __float_as_uint(vs1_now);
+        const bool normal = (bits & 0x7f800000u) != 0;
+        const float v_rest = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : (bits ? vs1_now * 0x1p126f : 1.f);
+        v_pow2 = normal || !bits ? __uint_as_float(bits & 0x7f800000u) : 0x1p-126f;
+        v_log2 = fast_log2(v_rest);
+        v_inv = __builtin_amdgcn_rcpf(v_rest);
+      }
+      bf16x8 hi[NT][U], lo[NT][U];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float c = SCALE == kScaleBlock ? ks1_now * k_factor : k_factor;
+        if (SCALE == kScaleToken || !clean) {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float x = s[n][j][r] * c;
+              if constexpr (SCALE == kScaleToken) x *= ks_now[j][r];
+              s[n][j][r] = clean || pos + 4 * j + r < limit[n] ? x : -INFINITY;  // (a select: bytes behind the context may be NaN)
+            }
+          }
+          c = 1.f;
+        }
+        float mx = s[n][0][0];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[n][j][r]);
+        }
+        mx = quad_row_max(mx * c);
+        if (__any(!(mx <= m_run[n] + kLag))) {
+          const float m_new = fmaxf(m_run[n], mx);
+          const float alpha = fast_exp2(m_run[n] - (m_new == -INFINITY ? 0.f : m_new));  // exp2(-inf) = 0 while the row has seen no key
+          m_run[n] = m_new;
+          l_run[n] *= alpha;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[n][db] *= alpha;
+        }
+        const float m_safe = m_run[n] == -INFINITY ? 0.f : m_run[n];
+        const float base = v_log2 - m_safe;
         float sum = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
           Bf16x8Bits ph, pl;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -305,9 +408,8 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int j = 2 * u + (w >> 1), r = 2 * (w & 1) + e;
-              p[e] = fast_exp2(s[n][j][r] - m_safe);
+              p[e] = fast_exp2(__builtin_fmaf(s[n][j][r], c, base));
               sum += p[e];
-              if constexpr (SCALE == kScaleBlock) p[e] *= vs1_now;
               if constexpr (SCALE == kScaleToken) p[e] *= vs_now[j][r];
             }
             ph.u[w] = pack_bf16x2(p[0], p[1]);
@@ -316,33 +418,14 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
           hi[n][u] = ph.v;
           lo[n][u] = pl.v;
         }
-        l_run[n] = l_run[n] * alpha + quad_row_sum(sum);
-        if (__any(alpha != 1.f)) {
-#pragma unroll
-          for (int db = 0; db < DB; ++db) acc[n][db] *= alpha;
-        }
+        l_run[n] += quad_row_sum(sum * v_inv);
       }
       // ---- O^T += V^T P --------------------------------------------------------------------------------------------------
-      // bytes behind the context may decode to NaN, and 0 * NaN is NaN: those tokens' V is zero
-      if (!clean && __any(live < 16)) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          vr[db][0] = keep_first_bytes(vr[db][0], FP8 ? live : 2 * live);
-          if constexpr (VL == 2) vr[db][1] = keep_first_bytes(vr[db][1], 2 * live - 16);
-        }
-      }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          bf16x8 v;
-          if constexpr (FP8) {
-            v = fp8x8_to_bf16x8(vr[db][0][2 * u], vr[db][0][2 * u + 1]);
-          } else {
-            Bf16x8Bits w;
-            w.u = vr[db][u];
-            v = w.v;
-          }
+        for (int u = 0; u < U; ++u) {
+          const bf16x8 v = v_operand(db, u, v_pow2);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             acc[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi[n][u], acc[n][db], 0, 0, 0);
@@ -361,7 +444,7 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
   // ---- the waves' results meet in LDS, one tile after the other ------------------------------------------------------------
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (n) __syncthreads();
+    if (n || Q_LDS) __syncthreads();
 #pragma unroll
     for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(&o_lds[wave][li][16 * db + 4 * kg]) = acc[n][db];
     if (kg == 0) {
@@ -545,7 +628,12 @@ int check_attention(const PaBlockArgs* a) {
   return PA_OK;
 }
 
-int row_tiles(const PaBlockArgs& a) { return a.group_size * a.q_len > 16 && a.head_size <= 128 ? 2 : 1; }
+// 16-row query tiles of a workgroup: as many as the call has, up to what the registers hold
+int row_tiles(const PaBlockArgs& a) {
+  const int tiles = (a.group_size * a.q_len + 15) / 16;
+  if (tiles == 1 || (a.head_size == 256 && a.kv_dtype == PA_DTYPE_BF16)) return 1;
+  return 2;
+}
 
 BlockCut choose_cut(const PaBlockArgs& a) {
   BlockCut c;
@@ -555,7 +643,7 @@ BlockCut choose_cut(const PaBlockArgs& a) {
   const int64_t axis = a.selected_blocks ? (int64_t)a.num_selected * a.block_size : c.axis;
   const int64_t units = (int64_t)a.num_seqs * a.num_kv_heads * c.row_groups;
   int64_t parts = (512 + units - 1) / units;             // two workgroups for each of 256 CUs
-  if (parts * 4096 < axis) parts = (axis + 4095) / 4096;  // a ragged batch's longest sequence is no tail of its own
+  if (parts * 4096 < axis) parts = (axis + 4096 - 1) / 4096;  // a ragged batch's longest sequence is no tail of its own
   if (parts > (axis + 255) / 256) parts = (axis + 255) / 256;
   if (parts < 1) parts = 1;
   const int64_t per = (axis + parts - 1) / parts;
@@ -573,19 +661,31 @@ int64_t workspace_of(const PaBlockArgs& a, const BlockCut& c) {
 }
 
 template <int D, bool FP8, int SCALE, int NT>
-int launch_stream(const PaBlockArgs& a, const BlockCut& c, dim3 grid, hipStream_t s) {
-  // (16-token blocks that one workgroup reads whole and nobody else reads: loads that do not stay in L2)
-  if (a.block_size == 16 && c.row_groups == 1)
-    return pa_launch(pa_block_attention_kernel<D, FP8, SCALE, NT, true>, grid, dim3(64 * kBlockWaves), 0, s, a, c);
-  return pa_launch(pa_block_attention_kernel<D, FP8, SCALE, NT, false>, grid, dim3(64 * kBlockWaves), 0, s, a, c);
+int launch_tile(const PaBlockArgs& a, const BlockCut& c, dim3 grid, hipStream_t s) {
+  // what a wave has in flight, the query operands and the accumulators share 256 registers (two waves per SIMD), or 512
+  constexpr int OCC = D == 256 && (!FP8 || NT > 1) ? 1 : 2;
+  constexpr int STEP = D == 256 || !FP8 || (D == 128 && SCALE == kScaleToken && NT > 1) ? 32 : 64;
+  constexpr bool Q_LDS = NT > 1 || D == 256;
+  // (16-token FP8 blocks that one workgroup reads whole and nobody else reads: loads that do not stay in L2)
+  if constexpr (FP8 && NT == 1)
+    if (a.block_size == 16 && c.row_groups == 1)
+      return pa_launch(pa_block_attention_kernel<D, FP8, SCALE, NT, STEP, OCC, Q_LDS, true>, grid, dim3(64 * kBlockWaves), 0, s, a, c);
+  return pa_launch(pa_block_attention_kernel<D, FP8, SCALE, NT, STEP, OCC, Q_LDS, false>, grid, dim3(64 * kBlockWaves), 0, s, a, c);
 }
 
-template <int D, int NT>
+template <int D, bool FP8, int SCALE>
+int launch_tiles(const PaBlockArgs& a, const BlockCut& c, dim3 grid, hipStream_t s) {
+  if constexpr (D < 256 || FP8)
+    if (row_tiles(a) == 2) return launch_tile<D, FP8, SCALE, 2>(a, c, grid, s);
+  return launch_tile<D, FP8, SCALE, 1>(a, c, grid, s);
+}
+
+template <int D>
 int launch_scale(const PaBlockArgs& a, const BlockCut& c, dim3 grid, hipStream_t s) {
-  if (a.kv_dtype == PA_DTYPE_BF16) return launch_stream<D, false, kScaleOne, NT>(a, c, grid, s);
-  if (a.kv_quant_mode == PA_QUANT_PER_TOKEN) return launch_stream<D, true, kScaleToken, NT>(a, c, grid, s);
-  if (a.kv_quant_mode == PA_QUANT_PER_BLOCK) return launch_stream<D, true, kScaleBlock, NT>(a, c, grid, s);
-  return launch_stream<D, true, kScaleOne, NT>(a, c, grid, s);
+  if (a.kv_dtype == PA_DTYPE_BF16) return launch_tiles<D, false, kScaleOne>(a, c, grid, s);
+  if (a.kv_quant_mode == PA_QUANT_PER_TOKEN) return launch_tiles<D, true, kScaleToken>(a, c, grid, s);
+  if (a.kv_quant_mode == PA_QUANT_PER_BLOCK) return launch_tiles<D, true, kScaleBlock>(a, c, grid, s);
+  return launch_tiles<D, true, kScaleOne>(a, c, grid, s);
 }
 
 }  // namespace
@@ -613,13 +713,9 @@ int pa_block_attention(const PaBlockArgs* a, void* hip_stream) {
   if (wgs > 0x7fffffffLL || rows > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
   hipStream_t s = reinterpret_cast<hipStream_t>(hip_stream);
   const dim3 grid((unsigned)wgs);
-  int rc;
-  if (a->head_size == 64)
-    rc = row_tiles(*a) == 2 ? launch_scale<64, 2>(*a, c, grid, s) : launch_scale<64, 1>(*a, c, grid, s);
-  else if (a->head_size == 128)
-    rc = row_tiles(*a) == 2 ? launch_scale<128, 2>(*a, c, grid, s) : launch_scale<128, 1>(*a, c, grid, s);
-  else
-    rc = launch_scale<256, 1>(*a, c, grid, s);
+  const int rc = a->head_size == 64    ? launch_scale<64>(*a, c, grid, s)
+                 : a->head_size == 128 ? launch_scale<128>(*a, c, grid, s)
+                                       : launch_scale<256>(*a, c, grid, s);
   if (rc || c.parts == 1) return rc;
   if (c.parts <= kFewParts) {
     const dim3 few((unsigned)((rows + 3) / 4));
