@@ -316,7 +316,7 @@ struct ScoreTile {
     ok = (unsigned)page < (unsigned)a.num_blocks;
     const __bf16* p = (const __bf16*)a.bounds + (int64_t)(ok ? page : 0) * a.stride_bounds_b + (int64_t)h * a.stride_bounds_h + 8 * (lane >> 4);
 #pragma unroll
-    for (int c = 0; c < 2 * KM; ++c) box[c] = load16_stream(p + 32 * c);
+    for (int c = 0; c < 2 * KM; ++c) box[c] = load16(p + 32 * c);  // (two loads share each 128-byte line: it has to stay in the cache)
   }
   __device__ __forceinline__ void score(const u32x4* q_lds, int tiles, int rows_valid, BlockScore* out, int at, int end, int lane) const {
     constexpr float kBound = 2 * D * 0x1p-23f;
@@ -367,17 +367,18 @@ __global__ __launch_bounds__(64 * kScoreWaves) void pa_block_score_kernel(const 
   extern __shared__ __attribute__((aligned(16))) u32x4 q_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunks = (axis_blocks + chunk - 1) / chunk;
-  const unsigned bh = blockIdx.x / (unsigned)chunks;
-  const int h = (int)(bh % (unsigned)a.num_kv_heads), b = (int)(bh / (unsigned)a.num_kv_heads);
+  const int h = (int)(blockIdx.x % (unsigned)a.num_kv_heads);
+  const unsigned at_chunk = blockIdx.x / (unsigned)a.num_kv_heads;
+  const int b = (int)(at_chunk / (unsigned)chunks);
+  const int begin = (int)(at_chunk % (unsigned)chunks) * chunk;
   const int nb = (block_context(a, b, axis) + a.block_size - 1) / a.block_size;
-  const int begin = (int)(blockIdx.x % (unsigned)chunks) * chunk;
   const int end = min(begin + chunk, nb - a.recent_blocks);
   if (nb <= a.num_selected || begin >= end) return;  // (every block is taken, or these blocks are: nobody reads their scores)
   int qb = a.q_lens ? a.q_lens[b] : a.q_len;
   qb = qb < 0 ? 0 : (qb > a.q_len ? a.q_len : qb);
   const int rows_valid = qb * a.group_size, tiles = (rows_valid + 15) / 16;
   const int* table = a.block_tables + (int64_t)b * a.stride_bt_s;
-  BlockScore* out = (BlockScore*)a.workspace + (int64_t)bh * axis_blocks;
+  BlockScore* out = (BlockScore*)a.workspace + ((int64_t)b * a.num_kv_heads + h) * axis_blocks;
   ScoreTile<D> t;
   int at = begin + 16 * wave;
   if (at < end) t.load(a, table, h, at, end, lane);
@@ -440,6 +441,7 @@ __device__ __forceinline__ unsigned long long exact_key(const PaBlockArgs& a, in
 // formed in 64 bits and the threshold is found by eight passes over the keys' bytes.
 // Bound by latency, not by bytes (8 per block, from L2).
 constexpr int kSelectThreads = 512;
+constexpr int kAhead = 4;
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kCandidates = 512;
@@ -501,11 +503,18 @@ __global__ __launch_bounds__(kSelectThreads) void pa_block_select_kernel(const P
   if (by_32 && want > 0) {
     // ---- range of s, largest e ----------------------------------------------------------------------------------------
     float mn = INFINITY, mx = -INFINITY, E = 0.f;
-    for (int i = begin + tid; i < end; i += kSelectThreads) {
-      const BlockScore v = score[i];
-      mn = fminf(mn, v.s);
-      mx = fmaxf(mx, v.s);
-      E = fmaxf(E, v.e);
+    // (kAhead scores of a thread are asked for at a time: one by one a pass would be a chain of L2 latencies; behind the end
+    // the last one is read again)
+    for (int i0 = begin + tid; i0 < end; i0 += kAhead * kSelectThreads) {
+      BlockScore v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) v[u] = score[min(i0 + u * kSelectThreads, end - 1)];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        mn = fminf(mn, v[u].s);
+        mx = fmaxf(mx, v[u].s);
+        E = fmaxf(E, v[u].e);
+      }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -535,7 +544,14 @@ __global__ __launch_bounds__(kSelectThreads) void pa_block_select_kernel(const P
         const float x = (s - mn) * scale;
         return x >= (float)(kBins - 1) ? kBins - 1 : (x > 0.f ? (int)x : 0);
       };
-      for (int i = begin + tid; i < end; i += kSelectThreads) atomicAdd(&hist[bin(score[i].s)], 1);
+      for (int i0 = begin + tid; i0 < end; i0 += kAhead * kSelectThreads) {
+        float v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = score[min(i0 + u * kSelectThreads, end - 1)].s;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (i0 + u * kSelectThreads < end) atomicAdd(&hist[bin(v[u])], 1);
+      }
       __syncthreads();
       // the bin in which the count from above reaches `want`: a thread owns four bins, the highest first
       constexpr int kOwn = kBins / kSelectThreads;
@@ -551,24 +567,32 @@ __global__ __launch_bounds__(kSelectThreads) void pa_block_select_kernel(const P
       __syncthreads();
       const int edge = found[0];
       // ---- taken, candidate or neither: a wave looks at 64 consecutive blocks ----------------------------------------------
-      for (int i0 = 64 * wave; i0 < nb; i0 += 64 * kSelectWaves) {
-        const int i = i0 + lane;
-        bool in = i < nb && (i < begin || i >= end), maybe = false;
-        if (i >= begin && i < end) {
-          const BlockScore v = score[i];
-          // (s +- (e + E), with room for the roundings here: e is at least 2^-16 of |s|)
-          const float slack = (v.e + E) * 1.01f;
-          in = bin(v.s - slack) > edge;
-          maybe = !in && bin(v.s + slack) >= edge;
-          if (in) atomicAdd(&num_in, 1);
+      int taken = 0;
+      for (int j0 = 64 * wave; j0 < nb; j0 += 64 * kSelectWaves * kAhead) {
+        BlockScore v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = j0 + 64 * kSelectWaves * u + lane;
+          v[u] = score[i < begin ? begin : min(i, end - 1)];
         }
-        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-        if (lane < 2) flags[(i0 >> 5) + lane] = (uint32_t)(mask >> (32 * lane));
-        if (maybe) {
-          const int at = atomicAdd(&num_cand, 1);
-          if (at < kCandidates) cand[at] = i;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i0 = j0 + 64 * kSelectWaves * u, i = i0 + lane;
+          if (i0 >= nb) break;
+          // (s +- (e + E), with room for the roundings here: e is at least 2^-16 of |s|)
+          const float slack = (v[u].e + E) * 1.01f;
+          const bool scored = i >= begin && i < end;
+          const bool in = scored && bin(v[u].s - slack) > edge;
+          const uint64_t above = __builtin_amdgcn_ballot_w64(in), ends = __builtin_amdgcn_ballot_w64(i < nb && !scored);
+          taken += __builtin_popcountll(above);
+          if (lane < 2) flags[(i0 >> 5) + lane] = (uint32_t)((above | ends) >> (32 * lane));
+          if (scored && !in && bin(v[u].s + slack) >= edge) {
+            const int at = atomicAdd(&num_cand, 1);
+            if (at < kCandidates) cand[at] = i;
+          }
         }
       }
+      if (lane == 0 && taken) atomicAdd(&num_in, taken);
       __syncthreads();
       by_32 = num_cand <= kCandidates;
     }
@@ -719,8 +743,8 @@ int pa_select_blocks(const PaBlockArgs* a, void* hip_stream) {
   hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
   const int axis = block_axis(*a), blocks = axis_blocks_of(*a);
   const int64_t heads = (int64_t)a->num_seqs * a->num_kv_heads;
-  // stretches long enough to pay for staging the query, short enough to fill the GPU: 64 blocks up to 2048 workgroups
-  int64_t chunk = (heads * blocks / 2048 + 63) / 64 * 64;
+  // stretches long enough to pay for staging the query, short enough to fill the GPU: 64 blocks up to 512 workgroups
+  int64_t chunk = (heads * blocks / 512 + 63) / 64 * 64;
   chunk = chunk < 64 ? 64 : (chunk > 1024 ? 1024 : chunk);
   const int64_t grid = heads * ((blocks + chunk - 1) / chunk);
   if (grid > 0x7fffffffLL) return PA_ERR_BAD_SHAPE;
