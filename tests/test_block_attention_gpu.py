@@ -77,7 +77,7 @@ def check(cuda, query, kc, vc, lens, table, q_len, ks, vs, selected=None, counts
     assert got is dev["out"]
     torch.cuda.synchronize()
     ref, lse, size = O.attention(query, kc, vc, lens, table, d ** -0.5, q_len, ks, vs, selected, counts, q_lens, max_len)
-    compare(dev["out"].cpu(), dev["lse"].cpu(), ref, lse, size, kc, vc, vs, table, max_len, d)
+    compare(dev["out"].cpu(), dev["lse"].cpu(), ref, lse, size, kc, vc, vs, table, min(max_len, table.shape[1] * kc.shape[3]), d)
     return dev["out"]
 
 
@@ -673,3 +673,30 @@ def test_an_empty_batch_is_no_error(cuda):
     T.key_block_bounds(box, kc, lens, table, 64)
     sel, cnt = T.select_blocks(q, box, lens, table, 3, 16, 1, 64)
     assert sel.shape == (0, 1, 3) and cnt.shape == (0, 1)
+
+
+def test_max_sequence_length_beyond_the_table_is_the_tables_reach(cuda):
+    """Serving code passes the model's longest context: the call is cut at what the block table holds."""
+    g = torch.Generator().manual_seed(21)
+    lens = torch.tensor([200, 48], dtype=torch.int32)
+    kc, vc, ks, vs = make_cache(g, 20, 2, 128, 16, "block")
+    table = make_table(g, lens, 16, 20)
+    query = torch.randn(2, 16, 128, generator=g).to(torch.bfloat16)
+    for longest in (200, 1 << 20, 1 << 40):
+        check(cuda, query, kc, vc, lens, table, 1, ks, vs, max_len=longest)
+        check_select(cuda, query, _box(g, 20, 2, 128), lens, table, 4, 16, 1, max_len=longest)
+    import triton_op_amd as T
+
+    got = torch.zeros(20, 2, 2, 128, dtype=torch.bfloat16)
+    want, dev = got.clone(), got.to(cuda)
+    T.key_block_bounds(dev, kc.to(cuda), lens.to(cuda), table.to(cuda), 1 << 40, ks.to(cuda))
+    O.bounds(want, kc, lens, table, ks)
+    assert torch.equal(dev.cpu(), want)
+
+
+def test_selection_without_a_query_row_takes_the_lowest_blocks(cuda):
+    g = torch.Generator().manual_seed(22)
+    lens = torch.tensor([16 * 30, 16 * 40], dtype=torch.int32)
+    box, table = _box(g, 80, 1, 64), make_table(g, lens, 16, 80)
+    query = torch.randn(2, 8, 64, generator=g).to(torch.bfloat16)
+    check_select(cuda, query, box, lens, table, 9, 16, 2, 1, 3, torch.tensor([0, 2], dtype=torch.int32))

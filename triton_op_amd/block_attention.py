@@ -232,7 +232,7 @@ def plan_block_attention(
         query_lens=query_lens, lse=lse, workspace=workspace))
     num_seqs, width, st_bt = _check_sequences(sequence_lengths, block_tables)
     code, x, blocks, heads, bs, head_size, st_kb, st_kh, st_kc = _check_key_cache(key_cache)
-    q_len, longest = int(query_sequence_length), max(0, int(max_sequence_length))
+    q_len, longest = int(query_sequence_length), max(0, min(int(max_sequence_length), width * bs))
     group, q_head_size, st_qs, st_qh = _check_query(query, q_len, heads, num_seqs, query_lens)
     if q_head_size != head_size:
         raise ValueError(f"query has head size {q_head_size}, key_cache {head_size}")
@@ -346,7 +346,7 @@ def key_block_bounds(
     st_bb, st_bh = _check_bounds(bounds)
     if bounds.shape != (blocks, heads, 2, head_size):
         raise ValueError(f"bounds shape {tuple(bounds.shape)} is not [{blocks}, {heads}, 2, {head_size}]")
-    new = 0 if new_tokens is None else int(new_tokens)
+    new, longest = 0 if new_tokens is None else int(new_tokens), max(0, min(int(max_sequence_length), width * bs))
     if new_tokens is not None and new < 1:
         raise ValueError(f"new_tokens must be positive, got {new_tokens}")
     if not bounds.is_cuda:
@@ -355,7 +355,7 @@ def key_block_bounds(
         args = PaBlockArgs.from_buffer_copy(_PACK.pack(
             _SIZE, 0,
             0, 0, key_cache.data_ptr(), 0, _ptr(key_scale), 0, sequence_lengths.data_ptr(), block_tables.data_ptr(), 0, bounds.data_ptr(), 0, 0, 0, 0,
-            num_seqs, heads, 0, 0, head_size, bs, blocks, width, max(0, int(max_sequence_length)), code, mode, 0, 0, 0, 0, min(new, 1 << 30),
+            num_seqs, heads, 0, 0, head_size, bs, blocks, width, longest, code, mode, 0, 0, 0, 0, min(new, 1 << 30),
             0.0, 0,
             0, 0, 0, 0, st_kb, st_kh, st_kc, 0, 0, 0, st_sb, st_sh, st_bt, st_bb, st_bh, 0, 0, 0, 0, 0))
         _launch("pa_block_bounds", args, index)
@@ -395,7 +395,8 @@ def select_blocks(
     blocks, heads, _, head_size = bounds.shape
     if blocks < 1 or heads < 1:
         raise ValueError(f"bounds shape {tuple(bounds.shape)} is empty")
-    q_len, longest, k, first = int(query_sequence_length), max(0, int(max_sequence_length)), int(num_selected), int(first_blocks)
+    q_len, longest = int(query_sequence_length), max(0, min(int(max_sequence_length), width * block_size))
+    k, first = int(num_selected), int(first_blocks)
     group, q_head_size, st_qs, st_qh = _check_query(query, q_len, heads, num_seqs, query_lens)
     if q_head_size != head_size:
         raise ValueError(f"query has head size {q_head_size}, bounds {head_size}")
