@@ -11,6 +11,8 @@
 // From there on a wave owns a (block, kv head) and needs no barrier: it goes through the block's 16-slot segments that
 // change, 16 bytes of a row per lane.  K leaves as 8-byte halves of (chunk, token) cells, V is turned in LDS so that a
 // head dim's 16 tokens are one 16-byte store, new codes among the old ones.  Every byte is written at most once.
+// Bound by the chain of latencies slot -> slot mapping -> rows -> store: 64 tokens x 8 heads 8 us, 8192 tokens (50 MB) 22 us = 2.3
+// TB/s; the read of the slot mapping grows with its square (65536 tokens: 255 us).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
