@@ -287,7 +287,7 @@ typedef struct PaKvWriteArgs {
   int32_t head_size;           /* 128; 64 and 256 are written token by token whatever num_tokens is */
   int32_t block_size;
   int32_t cache_dtype;         /* PA_DTYPE_* */
-  int32_t kv_quant_mode;       /* PA_QUANT_* */
+  int32_t kv_quant_mode;       /* PA_QUANT_*; PA_QUANT_PER_BLOCK in pa_kv_cache_write_block_scaled alone */
   int32_t v_transposed;        /* 0: value_cache [.., D, bs]; 1: [.., bs/x, D, x] (shuffle_value_cache_layout, test_pa_mtp.py:472-497) */
   int64_t stride_k_t, stride_k_h, stride_v_t, stride_v_h; /* elements; last dim contiguous */
   int64_t stride_kc_b, stride_kc_h, stride_vc_b, stride_vc_h; /* cache block / head strides; inner dims dense */

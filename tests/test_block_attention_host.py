@@ -234,6 +234,21 @@ def test_existing_entry_points_still_refuse_block_scales(pa_lib):
                       a["key_scale"], a["value_scale"])
 
 
+@pytest.mark.parametrize("mode", [2, 3, 7, -2, 1 << 20])
+def test_the_token_scaled_writer_refuses_other_modes(pa_lib, mode):
+    """pa_kv_cache_write knows no scale, one scale and one per token; with any other mode it would store codes that no scale
+    belongs to.  (No tokens: nothing could be launched, whatever the checks let through.)"""
+    w = _cabi.PaKvWriteArgs()
+    w.struct_size, w.num_tokens = C.sizeof(w), 0
+    for n in ("key", "value", "slot_mapping", "key_cache", "value_cache", "key_scale", "value_scale"):
+        setattr(w, n, 0x1000)
+    w.num_kv_heads, w.head_size, w.block_size, w.cache_dtype, w.kv_quant_mode = 2, 128, 16, _cabi.PA_DTYPE_FP8_E4M3FN, mode
+    assert pa_lib.pa_kv_cache_write(C.byref(w), None) == -3
+    for known in (_cabi.PA_QUANT_NONE, _cabi.PA_QUANT_PER_TENSOR, _cabi.PA_QUANT_PER_TOKEN):
+        w.kv_quant_mode = known
+        assert pa_lib.pa_kv_cache_write(C.byref(w), None) == 0
+
+
 # ---- the oracle ---------------------------------------------------------------------------------------------------------
 def test_oracle_attention_is_torchs():
     g = torch.Generator().manual_seed(0)

@@ -511,6 +511,8 @@ int pa_kv_cache_write(const PaKvWriteArgs* a, void* hip_stream) {
   if (a->num_tokens < 0 || a->num_kv_heads <= 0 || a->block_size <= 0) return PA_ERR_BAD_SHAPE;
   if (a->head_size != 128 && a->head_size != 64 && a->head_size != 256) return PA_ERR_UNSUPPORTED;
   if (a->cache_dtype != PA_DTYPE_BF16 && a->cache_dtype != PA_DTYPE_FP8_E4M3FN) return PA_ERR_UNSUPPORTED;
+  // (one scale per block is pa_kv_cache_write_block_scaled's: here its codes would be stored without a scale)
+  if (a->kv_quant_mode < PA_QUANT_NONE || a->kv_quant_mode > PA_QUANT_PER_TOKEN) return PA_ERR_UNSUPPORTED;
   if (a->v_transposed != 0 && a->v_transposed != 1) return PA_ERR_BAD_SHAPE;
   if (a->v_transposed && a->block_size % (a->cache_dtype == PA_DTYPE_FP8_E4M3FN ? 16 : 8)) return PA_ERR_BAD_SHAPE;
   if (a->cache_dtype == PA_DTYPE_FP8_E4M3FN && a->kv_quant_mode != PA_QUANT_NONE && (!a->key_scale || !a->value_scale))
