@@ -326,7 +326,8 @@ int pa_kv_cache_write_block_scaled(const PaKvWriteArgs* args, int64_t num_blocks
  * in PaDecodeArgs; N = num_blocks, W = table_width:
  *   output        bf16 [B, Hkv*Ge, D]          query  bf16 [B, Hkv*Ge, D]
  *   key_cache     [N, Hkv, D/x, bs, x]         value_cache [N, Hkv, D, bs] or transposed [N, Hkv, bs/x, D, x]
- *   key_scale, value_scale   by kv_quant_mode: none, one f32, [N, Hkv, bs, 1] or [N, Hkv, 1, 1]
+ *   key_scale, value_scale   by kv_quant_mode: none, one f32, [N, Hkv, bs, 1] or [N, Hkv, 1, 1]; finite, of either sign (those that
+ *                 pa_kv_cache_write_block_scaled keeps are never below zero)
  *   bounds        bf16 [N, Hkv, 2, D]          row 0 the smallest, row 1 the largest key of a block, per head dim
  *   selected_blocks  int32 [B, Hkv, K]         logical block numbers (positions in the sequence's row of block_tables)
  *   selected_counts  int32 [B, Hkv]            how many of them are meant

@@ -244,6 +244,29 @@ def test_attention_softmax_extremes(cuda, scale):
     compare(out.cpu(), lse.cpu(), ref, rlse, size, kc, vc, vs, table, 700, 128)
 
 
+def _with_signs(g, s):
+    return s * (2.0 * torch.randint(0, 2, s.shape, generator=g) - 1)
+
+
+@pytest.mark.parametrize("d,group,q_len,bs,vt", [(128, 8, 1, 16, False), (128, 16, 4, 16, False), (128, 5, 2, 1024, True), (64, 8, 1, 64, False),
+                                                 (64, 12, 3, 16, True), (256, 8, 1, 16, False), (256, 16, 2, 64, False)])
+@pytest.mark.parametrize("mode", ["block", "odd"])
+def test_attention_with_block_scales_of_either_sign(cuda, d, group, q_len, bs, vt, mode):
+    """Block scales below zero among the others, -0.0 and subnormal ones: a key or value is code * scale, whatever its sign.  The
+    queries are large enough that a softmax reference taken from the wrong end overflows."""
+    g = torch.Generator().manual_seed(d + group)
+    lens = torch.tensor([700, 64, 1, 2049, 17], dtype=torch.int32)
+    nblk = sum(-(-int(n) // bs) for n in lens) + 2
+    kc, vc, ks, vs = make_cache(g, nblk, 2, d, bs, mode, vt)
+    ks, vs = _with_signs(g, ks), _with_signs(g, vs)
+    table = make_table(g, lens, bs, nblk)
+    ks[table[0, 0], 0], vs[table[3, 1], 0] = -0.0, -0.0
+    vs[table[3, 2], 0], vs[table[0, 1] if bs < 1024 else table[1, 0], 1] = 2.0**-130, -(2.0**-131) * 1.5
+    query = torch.randn(len(lens), 2 * group * q_len, d, generator=g)
+    for size, k, v in ((4, ks, vs), (40, ks, vs), (40, -ks.abs(), -vs.abs())):
+        check(cuda, (size * query).to(torch.bfloat16), kc, vc, lens, table, q_len, k, v)
+
+
 # ---- selected blocks ------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("d,mode,bs,vt", [(128, "block", 16, False), (128, "bf16", 16, True), (64, "token", 64, False), (256, "block", 64, True),
                                           (128, "tensor", 1024, False)])

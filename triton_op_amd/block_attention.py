@@ -315,7 +315,7 @@ def paged_block_attention(
     counts twice).  Writes `output` (and `lse`, the natural logarithm of every row's softmax denominator) in place and
     returns `output`; rows that see no token, and rows beyond a sequence's `query_lens` entry, become zero (lse -inf).
     Contexts are cut at `max_sequence_length` and at the block table's width.  The value rows of a sequence's tokens
-    must be finite; what the cache holds behind a context does not matter."""
+    must be finite, and so must the scales, of either sign; what the cache holds behind a context does not matter."""
     plan = plan_block_attention(
         output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale, query_sequence_length,
         max_sequence_length, key_scale, value_scale, selected_blocks=selected_blocks, selected_counts=selected_counts,

@@ -338,7 +338,9 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
       }
       // ---- softmax (s[n][j][r]: token 4 j + r of the lane's) --------------------------------------------------------------
       const int pos = pick(now.pos, kg) + inside(kg);
-      const bool clean = __all(pos + TPL <= limit_all);
+      bool plain = pos + TPL <= limit_all;
+      if constexpr (SCALE == kScaleBlock) plain = plain && !(fminf(ks1_now, vs1_now) < 0.f);  // (a scale below zero turns the order of the logits)
+      const bool clean = __all(plain);
       const int live = ctx - pos;  // live tokens of the lane's (may be <= 0 or >= TPL)
       if (!clean) {  // a scale behind the context may be NaN, and 0 * NaN is NaN
         if constexpr (SCALE == kScaleBlock) vs1_now = live > 0 ? vs1_now : 0.f;
@@ -360,14 +362,25 @@ void pa_block_attention_kernel(const PaBlockArgs a, const BlockCut cut) {
             }
           }
         }
+        // the sign of V's scale goes to the codes
+        if constexpr (SCALE == kScaleBlock) {
+          if (__any(vs1_now < 0.f)) {
+            const uint32_t turn = vs1_now < 0.f ? 0x80808080u : 0u;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+#pragma unroll
+              for (int w = 0; w < VW; ++w) vr[db][w] ^= turn;
+            }
+          }
+        }
       }
-      // V's scale is 2^e v_rest with v_rest in [1, 2): the power is applied when the codes are converted, v_rest as a summand of
-      // the probabilities' exponents, which the lane's sum is rid of again (both are exactly nothing for a power of two)
+      // The size of V's scale is 2^e v_rest with v_rest in [1, 2): the power is applied when the codes are converted, v_rest as a
+      // summand of the probabilities' exponents, which the lane's sum is rid of again (both are exactly nothing for a power of two)
       float v_pow2 = 1.f, v_log2 = 0.f, v_inv = 1.f;
       if constexpr (SCALE == kScaleBlock) {
-        const uint32_t bits = __float_as_uint(vs1_now);
+        const uint32_t bits = __float_as_uint(vs1_now) & 0x7fffffffu;
         const bool normal = (bits & 0x7f800000u) != 0;
-        const float v_rest = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : (bits ? vs1_now * 0x1p126f : 1.f);
+        const float v_rest = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : (bits ? __uint_as_float(bits) * 0x1p126f : 1.f);
         v_pow2 = normal || !bits ? __uint_as_float(bits & 0x7f800000u) : 0x1p-126f;
         v_log2 = fast_log2(v_rest);
         v_inv = __builtin_amdgcn_rcpf(v_rest);

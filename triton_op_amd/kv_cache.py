@@ -82,7 +82,7 @@ def kv_cache_write(
 ) -> None:
     """New tokens into their slots.  With scales [blocks, Hkv, 1, 1] a block's codes share one scale per head: it only
     grows, by powers of two, and the codes that are already in the block follow it (set a block's scales to 0 when it is
-    handed to another sequence: 0 marks an empty block); of two tokens with one slot the later one stays, and slots
+    handed to another sequence: 0 marks an empty block; no scale may be below 0 or not finite); of two tokens with one slot the later one stays, and slots
     outside the cache are skipped."""
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16 or key.shape != value.shape or key.dim() != 3:
         raise ValueError("key and value must be bfloat16 [num_tokens, num_kv_heads, head_size]")
