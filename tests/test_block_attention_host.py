@@ -143,6 +143,50 @@ def test_write_refuses_what_its_scales_do_not_fit(monkeypatch):
             KC.kv_cache_write(**{**good, **over})
 
 
+@pytest.mark.parametrize("call,over", [
+    (_attention, dict(output=_z(1, 8, 128, dtype=torch.bfloat16).expand(2, 8, 128))),
+    (_attention, dict(output=_z(2, 1, 128, dtype=torch.bfloat16).expand(2, 8, 128))),
+    (_attention, dict(lse=_z(1, 8).expand(2, 8))),
+    (_bounds, dict(bounds=_z(9, 1, 2, 128, dtype=torch.bfloat16).expand(9, 2, 2, 128))),
+    (_bounds, dict(bounds=_z(1, 2, 2, 128, dtype=torch.bfloat16).expand(9, 2, 2, 128))),
+    (_select, dict(selected_blocks=_z(2, 1, 2, dtype=torch.int32).expand(2, 2, 2))),
+    (_select, dict(selected_counts=_z(1, 2, dtype=torch.int32).expand(2, 2))),
+])
+def test_written_tensors_must_not_be_expanded(call, over):
+    """Several results for one place: what is left there would depend on which workgroup comes last."""
+    entry = {_attention: T.paged_block_attention, _bounds: T.key_block_bounds, _select: T.select_blocks}[call]
+    with pytest.raises(ValueError, match="must not be an expanded tensor"):
+        entry(**call(**over))
+
+
+def test_expanded_tensors_that_are_only_read_are_fine():
+    one = _z(1, 1, 1, 1)
+    for call, entry, over in (
+            (_attention, T.paged_block_attention, dict(key_scale=one.expand(9, 2, 1, 1), value_scale=one.expand(9, 2, 1, 1))),
+            (_attention, T.paged_block_attention, dict(block_tables=_z(1, 3, dtype=torch.int32).expand(2, 3), lse=_z(2, 8),
+                                                       selected_blocks=_z(2, 1, 5, dtype=torch.int32).expand(2, 2, 5))),
+            (_bounds, T.key_block_bounds, dict(key_scale=one.expand(9, 2, 1, 1))),
+            (_select, T.select_blocks, dict(bounds=_z(1, 2, 2, 128, dtype=torch.bfloat16).expand(9, 2, 2, 128)))):
+        with pytest.raises(ValueError, match="GPU only"):
+            entry(**call(**over))
+
+
+def test_write_refuses_scales_that_share_their_memory(monkeypatch):
+    """A head's scale decides its codes: heads (or K and V) that write one scale each into the same place leave codes without theirs."""
+    from triton_op_amd import kv_cache as KC
+
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    key = _z(3, 2, 128, dtype=torch.bfloat16)
+    good = dict(key=key, value=key, key_cache=_z(9, 2, 8, 16, 16).to(FP8), value_cache=_z(9, 2, 128, 16).to(FP8),
+                slot_mapping=torch.zeros(3, dtype=torch.int64), key_scale=_z(9, 2, 1, 1), value_scale=_z(9, 2, 1, 1))
+    per_block = dict(key_scale=_z(9, 1, 1, 1).expand(9, 2, 1, 1), value_scale=_z(9, 1, 1, 1).expand(9, 2, 1, 1))
+    same = dict(key_scale=good["key_scale"], value_scale=good["key_scale"])
+    cache = dict(key_cache=_z(1, 2, 8, 16, 16).to(FP8).expand(9, 2, 8, 16, 16))
+    for over, msg in ((per_block, "expanded"), (same, "same memory"), (cache, "expanded")):
+        with pytest.raises(ValueError, match=msg):
+            KC.kv_cache_write(**{**good, **over})
+
+
 def test_struct_matches_the_header(pa_lib):
     with open(os.path.join(ROOT, "include", "pa_decode.h")) as f:
         body = re.search(r"typedef struct PaBlockArgs \{(.*?)\} PaBlockArgs;", f.read(), re.S).group(1)

@@ -22,7 +22,7 @@ import torch
 
 from . import _cabi
 from ._cabi import PaBlockArgs
-from .kv_cache import FP8_DTYPE, _current_raw_stream, _strides
+from .kv_cache import FP8_DTYPE, _check_written, _current_raw_stream, _strides
 
 _SUPPORTED_BLOCK_SIZES = (16, 64, 1024)
 _SUPPORTED_HEAD_SIZES = (64, 128, 256)
@@ -272,6 +272,7 @@ def plan_block_attention(
         if lse.dtype is not torch.float32 or lse.shape != query.shape[:2] or lse.stride(1) != 1:
             raise ValueError(f"lse must be float32 {tuple(query.shape[:2])}, dense over the rows")
         st_lse = lse.stride(0)
+    _check_written(output=output, lse=lse)
     if not output.is_cuda:
         raise ValueError("paged_block_attention runs on the GPU only (there is no CPU path); got a CPU tensor")
     if num_seqs:
@@ -346,6 +347,7 @@ def key_block_bounds(
     st_bb, st_bh = _check_bounds(bounds)
     if bounds.shape != (blocks, heads, 2, head_size):
         raise ValueError(f"bounds shape {tuple(bounds.shape)} is not [{blocks}, {heads}, 2, {head_size}]")
+    _check_written(bounds=bounds)
     new, longest = 0 if new_tokens is None else int(new_tokens), max(0, min(int(max_sequence_length), width * bs))
     if new_tokens is not None and new < 1:
         raise ValueError(f"new_tokens must be positive, got {new_tokens}")
@@ -408,6 +410,7 @@ def select_blocks(
         raise ValueError(f"num_selected == {num_selected} does not hold first_blocks + recent_blocks == {first_blocks} + {recent}")
     if k * block_size > 1 << 30:
         raise ValueError(f"num_selected == {num_selected} blocks of {block_size} tokens are too many")
+    _check_written(selected_blocks=selected_blocks, selected_counts=selected_counts)
     if not query.is_cuda:
         raise ValueError("select_blocks runs on the GPU only (there is no CPU path); got a CPU tensor")
     if selected_blocks is None:

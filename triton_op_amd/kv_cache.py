@@ -36,6 +36,13 @@ def _strides(t: torch.Tensor) -> Tuple[int, ...]:
     return tuple(st if n > 1 else 0 for n, st in zip(t.shape, t.stride()))
 
 
+def _check_written(**tensors: Optional[torch.Tensor]) -> None:
+    """Tensors a call writes: an expanded one has one place for results that differ, and which of them stays is chance."""
+    for name, t in tensors.items():
+        if t is not None and 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+            raise ValueError(f"{name} is written and must not be an expanded tensor")
+
+
 def quantize_kv_cache_symmetric(
     key_cache: torch.Tensor,    # [num_blocks, num_heads, head_size // 8, block_size, 8] bf16
     value_cache: torch.Tensor,  # [num_blocks, num_heads, head_size, block_size] bf16
@@ -128,6 +135,9 @@ def kv_cache_write(
         elif tuple(key_scale.shape) == (key_cache.shape[0], h, 1, 1) and bs != 1:
             if _strides(key_scale) != _strides(value_scale):
                 raise ValueError("key_scale and value_scale must have the same strides")
+            _check_written(key_scale=key_scale, value_scale=value_scale, key_cache=key_cache, value_cache=value_cache)
+            if key_scale.data_ptr() == value_scale.data_ptr() and key_cache.shape[0]:
+                raise ValueError("key_scale and value_scale are written and must not be the same memory")
             mode = _cabi.PA_QUANT_PER_BLOCK
             st_sb, st_sh = key_scale.stride(0), key_scale.stride(1)
         else:
