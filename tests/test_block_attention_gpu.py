@@ -331,6 +331,32 @@ def test_bounds(cuda, d, mode, bs):
         assert torch.equal(dev.cpu().view(torch.int16) & 0x7fff, want.view(torch.int16) & 0x7fff) and torch.equal(dev.cpu(), want)
 
 
+@pytest.mark.parametrize("mode", ["block", "tensor", "token"])
+@pytest.mark.parametrize("bs", [16, 64])
+def test_bounds_with_scales_of_either_sign_and_zero(cuda, mode, bs):
+    """A negative scale turns the smallest code into the largest key; a head dim without a number has no bounds (+infinity,
+    -infinity) whatever the scale is, zero too."""
+    import triton_op_amd as T
+
+    g = torch.Generator().manual_seed(bs)
+    lens = torch.tensor([5 * bs - 3, 1, bs], dtype=torch.int32)
+    kc, _, ks, _ = make_cache(g, 8, 3, 128, bs, mode)
+    kf = kc.float()
+    kf[:, 1, 0, :, 3], kf[:, 2, 3, :, 0] = math.nan, math.nan
+    kc = kf.to(kc.dtype)
+    table = make_table(g, lens, bs, 8)
+    signed = [_with_signs(g, ks), -ks.abs(), torch.zeros_like(ks), -torch.zeros_like(ks)]
+    if ks.dim():
+        signed.append(_with_signs(g, ks) * torch.randint(0, 2, ks.shape, generator=g))
+    for s in signed:
+        want = torch.full((8, 3, 2, 128), 5.0, dtype=torch.bfloat16)
+        dev = want.to(cuda)
+        T.key_block_bounds(dev, kc.to(cuda), lens.to(cuda), table.to(cuda), int(lens.max()), s.to(cuda))
+        O.bounds(want, kc, lens, table, s)
+        torch.cuda.synchronize()
+        assert torch.equal(dev.cpu(), want)
+
+
 def test_bounds_of_strided_tensors_and_bad_entries(cuda):
     import triton_op_amd as T
 

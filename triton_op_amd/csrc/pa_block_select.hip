@@ -224,12 +224,17 @@ __global__ __launch_bounds__(256) void pa_block_bounds_kernel(const PaBlockArgs 
     const bool is_hi = base >= HALF;
     const float sign = is_hi ? scale : -scale;
     // (a negative scale turns the smallest code into the largest key)
-    __bf16* out = (__bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)(h0 + g) * a.stride_bounds_h + (is_hi != (scale < 0.f) ? D : 0) +
+    const bool row_hi = is_hi != (scale < 0.f);
+    const float none = row_hi ? -INFINITY : INFINITY;  // a head dim without a key that is a number, whatever the scale (0 * infinity is NaN)
+    __bf16* out = (__bf16*)a.bounds + (int64_t)page * a.stride_bounds_b + (int64_t)(h0 + g) * a.stride_bounds_h + (row_hi ? D : 0) +
                   lane / LPC * X + (is_hi ? base - HALF : base) * Slot::kDims;
     constexpr int N = KEEP * Slot::kDims;  // consecutive head dims
     uint32_t bits[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) bits[i] = __builtin_bit_cast(uint16_t, (__bf16)(slot[i / Slot::kDims].dim(i % Slot::kDims) * sign));
+    for (int i = 0; i < N; ++i) {
+      const float x = slot[i / Slot::kDims].dim(i % Slot::kDims);
+      bits[i] = __builtin_bit_cast(uint16_t, (__bf16)(x == -INFINITY ? none : x * sign));
+    }
     if constexpr (N == 1) {
       *reinterpret_cast<uint16_t*>(out) = (uint16_t)bits[0];
     } else {
