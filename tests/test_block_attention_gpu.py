@@ -453,6 +453,42 @@ def test_selection_with_bounds_that_are_no_numbers(cuda):
         check_select(cuda, query, box, lens, table, k, 16, 1, 1, 2)
 
 
+def test_selection_from_more_blocks_than_the_flags_hold(cuda):
+    """More than 65536 blocks (a million tokens in blocks of 16): every score is formed in 64 bits."""
+    g = torch.Generator().manual_seed(13)
+    n = 65536 + 777
+    lens = torch.tensor([16 * n - 5, 16 * 3000], dtype=torch.int32)
+    box, table = _box(g, n, 1, 64), torch.stack([torch.randperm(n, generator=g), torch.randint(0, n, (n,), generator=g)]).to(torch.int32)
+    table[0, 70] = -1
+    query = torch.randn(2, 2, 64, generator=g).to(torch.bfloat16)
+    for k, first, recent in ((300, 1, 2), (3, 1, 2), (20000, 0, 1)):
+        check_select(cuda, query, box, lens, table, k, 16, 1, first, recent)
+    check_select(cuda, torch.cat([query, query], 1), box, lens, table, 9, 16, 2, 1, 3, torch.tensor([0, 1], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("size", [3.0, 30.0, 100.0, 1.0e6])
+@pytest.mark.parametrize("k", [256, 1024, 4096])
+def test_selection_with_one_block_of_large_keys(cuda, size, k):
+    """The first block's keys are often the largest by far.  They widen the 32-bit stage's intervals and errors, so that many or
+    all blocks are left to the 64-bit stage."""
+    g = torch.Generator().manual_seed(14)
+    n = 8192
+    box, table = _box(g, n, 1, 128), torch.randperm(n, generator=g).to(torch.int32)[None]
+    box[table[0, 0].long()] *= size
+    query = torch.randn(1, 8, 128, generator=g).to(torch.bfloat16)
+    check_select(cuda, query, box, torch.tensor([16 * n], dtype=torch.int32), table, k, 16, 1)
+
+
+def test_selection_of_the_largest_rows(cuda):
+    """64 query rows of head size 256: the query operands fill the 64 KiB of LDS that a launch may ask for."""
+    g = torch.Generator().manual_seed(15)
+    lens = torch.tensor([64 * 150 - 1, 64 * 20, 70], dtype=torch.int32)
+    box, table = _box(g, 180, 2, 256), make_table(g, lens, 64, 180)
+    query = torch.randn(3, 2 * 64, 256, generator=g).to(torch.bfloat16)
+    for q_len in (1, 4):
+        check_select(cuda, query, box, lens, table, 17, 64, q_len, 1)
+
+
 def test_selection_into_the_callers_tensors(cuda):
     g = torch.Generator().manual_seed(12)
     lens = torch.tensor([16 * 30, 100], dtype=torch.int32)
