@@ -210,6 +210,39 @@ def test_attention_of_strided_tensors(cuda):
     assert bool(rest[:, 0].isnan().all()) and bool(rest[:, :, d:].isnan().all())  # nothing beside the rows was written
 
 
+def test_one_of_everything_with_strides_that_mean_nothing(cuda):
+    """One sequence, head, row and block: the strides of those dimensions may be any number, in each of the operators."""
+    import triton_op_amd as T
+
+    def odd(t, *dims):
+        return t.as_strided(t.shape, [7 if i in dims else st for i, st in enumerate(t.stride())])
+
+    g = torch.Generator().manual_seed(23)
+    lens, table = torch.tensor([13], dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    query = torch.randn(1, 1, 128, generator=g).to(torch.bfloat16)
+    for mode in ("block", "token"):
+        kc, vc, ks, vs = make_cache(g, 1, 1, 128, 16, mode, True)
+        one = (0, 1, 2) if mode == "block" else (0, 1)
+        check(cuda, query, kc, vc, lens, table, 1, ks, vs, gpu=dict(
+            query=odd(query.to(cuda), 0, 1), kc=odd(kc.to(cuda), 0, 1), vc=odd(vc.to(cuda), 0, 1, 2), ks=odd(ks.to(cuda), *one), vs=odd(vs.to(cuda), *one),
+            out=odd(torch.zeros(1, 1, 128, dtype=torch.bfloat16, device=cuda), 0, 1), lse=odd(torch.zeros(1, 1, device=cuda), 0, 1),
+            table=odd(table.to(cuda), 0, 1)))
+        want = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16)
+        box = odd(want.to(cuda), 0, 1)
+        T.key_block_bounds(box, odd(kc.to(cuda), 0, 1), lens.to(cuda), odd(table.to(cuda), 0, 1), 13, odd(ks.to(cuda), *one))
+        O.bounds(want, kc, lens, table, ks)
+        assert torch.equal(box.cpu(), want)
+        sel, cnt = T.select_blocks(odd(query.to(cuda), 0, 1), box, lens.to(cuda), table.to(cuda), 1, 16, 1, 13)
+        assert sel.tolist() == [[[0]]] and cnt.tolist() == [[1]]
+    key, value = _rows(g, 5, 1, 128)
+    host = [torch.zeros(1, 1, 8, 16, 16).to(FP8), torch.zeros(1, 1, 1, 128, 16).to(FP8), torch.zeros(1, 1, 1, 1), torch.zeros(1, 1, 1, 1)]
+    dev = [odd(t.to(cuda), *dims) for t, dims in zip(host, ((0, 1), (0, 1), (0, 1, 2), (0, 1)))]
+    T.kv_cache_write(key.to(cuda), value.to(cuda), dev[0], dev[1], torch.arange(5, device=cuda), dev[2], dev[3])
+    O.write(key, value, *host[:2], torch.arange(5), *host[2:])
+    for a, b in zip(dev, host):
+        assert torch.equal(a.cpu().float(), b.float())
+
+
 def test_attention_in_a_cache_beyond_32_bit_offsets(cuda):
     """Blocks at both ends of a cache of more than 2^32 bytes."""
     g = torch.Generator().manual_seed(6)

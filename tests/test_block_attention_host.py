@@ -171,6 +171,32 @@ def test_expanded_tensors_that_are_only_read_are_fine():
             entry(**call(**over))
 
 
+def _odd(t, *dims):
+    """The tensor with strides that mean nothing (odd ones) in dimensions of size 1."""
+    st = list(t.stride())
+    for i in dims:
+        assert t.shape[i] == 1
+        st[i] = 7
+    return t.as_strided(t.shape, st)
+
+
+def test_strides_of_dimensions_of_size_one_mean_nothing():
+    b16 = dict(dtype=torch.bfloat16)
+    one = dict(output=_odd(_z(1, 1, 128, **b16), 0, 1), query=_odd(_z(1, 1, 128, **b16), 0, 1), key_cache=_odd(_z(1, 1, 8, 16, 16).to(FP8), 0, 1),
+               value_cache=_odd(_z(1, 1, 1, 128, 16).to(FP8), 0, 1, 2), sequence_lengths=torch.tensor([9], dtype=torch.int32),
+               block_tables=_odd(_z(1, 1, dtype=torch.int32), 0, 1), key_scale=_odd(_z(1, 1, 16, 1), 0, 1), value_scale=_odd(_z(1, 1, 16, 1), 0, 1),
+               lse=_odd(_z(1, 1), 0, 1), selected_blocks=_odd(_z(1, 1, 1, dtype=torch.int32), 0, 1, 2),
+               selected_counts=_odd(_z(1, 1, dtype=torch.int32), 0, 1))
+    for over in ({}, dict(key_scale=_odd(_z(1, 1, 1, 1), 0, 1), value_scale=_odd(_z(1, 1, 1, 1), 0, 1, 2))):
+        with pytest.raises(ValueError, match="GPU only"):
+            T.paged_block_attention(**_attention(**{**one, **over}))
+    box = _odd(_z(1, 1, 2, 128, **b16), 0, 1)
+    with pytest.raises(ValueError, match="GPU only"):
+        T.key_block_bounds(**_bounds(bounds=box, **{n: one[n] for n in ("key_cache", "sequence_lengths", "block_tables", "key_scale")}))
+    with pytest.raises(ValueError, match="GPU only"):
+        T.select_blocks(**_select(bounds=box, num_selected=1, **{n: one[n] for n in ("query", "sequence_lengths", "block_tables")}))
+
+
 def test_write_refuses_scales_that_share_their_memory(monkeypatch):
     """A head's scale decides its codes: heads (or K and V) that write one scale each into the same place leave codes without theirs."""
     from triton_op_amd import kv_cache as KC

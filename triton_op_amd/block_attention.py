@@ -82,6 +82,8 @@ def _check_query(query, q_len: int, num_kv_heads: int, num_seqs: int, query_lens
     if head_size not in _SUPPORTED_HEAD_SIZES:
         raise ValueError(f"head_size == {head_size} is not supported (64, 128 or 256)")
     st = query.stride()
+    if st[0] % 8 or st[1] % 8:
+        st = _strides(query)
     if st[2] != 1 or st[0] % 8 or st[1] % 8 or query.data_ptr() % 16:
         raise ValueError("query rows must be dense and 16-byte aligned")
     if query_lens is not None and (query_lens.dtype is not torch.int32 or query_lens.numel() != seqs or not query_lens.is_contiguous()):
@@ -111,6 +113,8 @@ def _check_key_cache(key_cache):
         raise ValueError(f"key_cache shape {tuple(shape)} is not [blocks, kv_heads, head_size//{x}, bs, {x}] "
                          "with a head size of 64, 128 or 256")
     s0, s1, s2, s3, s4 = key_cache.stride()
+    if s0 % x or s1 % x:
+        s0, s1 = _strides(key_cache)[:2]
     if s4 != 1 or s3 != x or s0 % x or s1 % x or s2 % x or key_cache.data_ptr() % 16:
         raise ValueError("the innermost dimensions of key_cache must be dense and 16-byte aligned")
     return code, x, blocks, heads, bs, chunks * x, s0, s1, s2
@@ -136,6 +140,8 @@ def _check_scales(code: int, blocks: int, heads: int, bs: int, key_scale, value_
         return _cabi.PA_QUANT_PER_BLOCK, st[0], st[1]
     if shape != (blocks, heads, bs, 1):
         raise ValueError(f"Expected scales of shape [], [{blocks}, {heads}, 1, 1] or [{blocks}, {heads}, {bs}, 1], got {shape}")
+    if st[0] % 4 or st[1] % 4:
+        st = _strides(key_scale)
     if st[2] != 1 or st[0] % 4 or st[1] % 4 or key_scale.data_ptr() % 16 or (both and value_scale.data_ptr() % 16):
         raise ValueError("per-token scales must be dense over tokens and 16-byte aligned")
     return _cabi.PA_QUANT_PER_TOKEN, st[0], st[1]
@@ -147,6 +153,8 @@ def _check_bounds(bounds) -> Tuple[int, int]:
     if bounds.dtype is not torch.bfloat16 or len(shape) != 4 or shape[2] != 2:
         raise ValueError("bounds must be bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
     s0, s1, s2, s3 = bounds.stride()
+    if s0 % 8 or s1 % 8:
+        s0, s1 = _strides(bounds)[:2]
     if s3 != 1 or s2 != shape[3] or s0 % 8 or s1 % 8 or bounds.data_ptr() % 16:
         raise ValueError("the two bounds of a (block, head) must be dense and 16-byte aligned")
     return s0, s1
@@ -239,6 +247,8 @@ def plan_block_attention(
     if output.shape != query.shape or output.dtype is not torch.bfloat16:
         raise ValueError(f"output must be bfloat16 {tuple(query.shape)}, got {output.dtype} {tuple(output.shape)}")
     st_os, st_oh, st_od = output.stride()
+    if st_os % 4 or st_oh % 4:
+        st_os, st_oh, _ = _strides(output)
     if st_od != 1 or st_os % 4 or st_oh % 4 or output.data_ptr() % 8:
         raise ValueError("output rows must be dense and 8-byte aligned")
     # ---- value cache ---------------------------------------------------------------------------------------------------
@@ -249,6 +259,8 @@ def plan_block_attention(
         raise ValueError(f"value_cache shape {tuple(value_cache.shape)} is not [blocks, kv_heads, D, bs] or, transposed, "
                          f"[blocks, kv_heads, bs/{x}, D, {x}] of the key cache")
     st_v = value_cache.stride()
+    if st_v[0] % x or st_v[1] % x or st_v[2] % x:
+        st_v = _strides(value_cache)
     if st_v[-1] != 1 or (v_transposed and st_v[3] != x) or st_v[0] % x or st_v[1] % x or st_v[2] % x or value_cache.data_ptr() % 16:
         raise ValueError("the innermost dimensions of value_cache must be dense and 16-byte aligned")
     mode, st_sb, st_sh = _check_scales(code, blocks, heads, bs, key_scale, value_scale, True)
@@ -269,7 +281,7 @@ def plan_block_attention(
             raise ValueError(f"selected_counts must be int32 [{num_seqs}, {heads}], dense over the heads")
         st_cs = selected_counts.stride(0)
     if lse is not None:
-        if lse.dtype is not torch.float32 or lse.shape != query.shape[:2] or lse.stride(1) != 1:
+        if lse.dtype is not torch.float32 or lse.shape != query.shape[:2] or (lse.stride(1) != 1 and lse.shape[1] > 1):
             raise ValueError(f"lse must be float32 {tuple(query.shape[:2])}, dense over the rows")
         st_lse = lse.stride(0)
     _check_written(output=output, lse=lse)

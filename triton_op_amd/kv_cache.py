@@ -147,6 +147,8 @@ def kv_cache_write(
             mode = _cabi.PA_QUANT_PER_TOKEN
             st_sb, st_sh = key_scale.stride(0), key_scale.stride(1)
     st_kc, st_vc = key_cache.stride(), value_cache.stride()
+    if mode == _cabi.PA_QUANT_PER_BLOCK and (st_kc[0] % 16 or st_kc[1] % 16 or st_vc[0] % 16 or st_vc[1] % 16):
+        st_kc, st_vc = _strides(key_cache), _strides(value_cache)
     a = PaKvWriteArgs.from_buffer_copy(_PACK.pack(
         _PACK.size, 0,
         key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
