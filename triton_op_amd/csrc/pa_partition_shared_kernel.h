@@ -1,10 +1,24 @@
-// pa_partition_shared_kernel: stage 1 for 17..64 query rows per kv head over an FP8 cache.
+// pa_partition_shared_kernel: stage 1 for 17..64 query rows per kv head over an FP8 cache.  Included by pa_decode.hip alone
+// (pa_trace is one array per translation unit).
 #ifndef PA_PARTITION_SHARED_KERNEL_H_
 #define PA_PARTITION_SHARED_KERNEL_H_
 
 #include "pa_common.h"
 
 namespace {
+
+// -DPA_DECODE_TRACE (the measuring build tests/native/libpa_decode_trace.so, never the product library): one wave of
+// every workgroup of pa_partition_shared_kernel leaves six timestamps of the 100 MHz wall clock, its step count
+// and its live rows in pa_trace; pa_decode_trace_read copies them out.  PA_TRACE_MARK(i) is nothing otherwise.
+#ifdef PA_DECODE_TRACE
+constexpr int kTraceWorkgroups = 16384;
+__device__ unsigned long long pa_trace[kTraceWorkgroups * 8];
+#define PA_TRACE_DECL unsigned long long pa_trace_t[6] = {0, 0, 0, 0, 0, 0}
+#define PA_TRACE_MARK(i) pa_trace_t[i] = wall_clock64()
+#else
+#define PA_TRACE_DECL
+#define PA_TRACE_MARK(i)
+#endif
 
 // ---------------------------------------------------------------------------------------------
 // Partition kernel for more than 16 query rows per kv head (large GQA groups, MTP) over an FP8 cache.
