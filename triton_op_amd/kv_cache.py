@@ -89,8 +89,8 @@ def kv_cache_write(
 ) -> None:
     """New tokens into their slots.  With scales [blocks, Hkv, 1, 1] a block's codes share one scale per head: it only
     grows, by powers of two, and the codes that are already in the block follow it (set a block's scales to 0 when it is
-    handed to another sequence: 0 marks an empty block; no scale may be below 0 or not finite); of two tokens with one slot the later one stays, and slots
-    outside the cache are skipped."""
+    handed to another sequence: 0 marks an empty block; no scale may be below 0 or not finite); of two tokens with one
+    slot the later one stays, and slots outside the cache are skipped."""
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16 or key.shape != value.shape or key.dim() != 3:
         raise ValueError("key and value must be bfloat16 [num_tokens, num_kv_heads, head_size]")
     if not key.is_cuda:
@@ -135,9 +135,6 @@ def kv_cache_write(
         elif tuple(key_scale.shape) == (key_cache.shape[0], h, 1, 1) and bs != 1:
             if _strides(key_scale) != _strides(value_scale):
                 raise ValueError("key_scale and value_scale must have the same strides")
-            _check_written(key_scale=key_scale, value_scale=value_scale, key_cache=key_cache, value_cache=value_cache)
-            if key_scale.data_ptr() == value_scale.data_ptr() and key_cache.shape[0]:
-                raise ValueError("key_scale and value_scale are written and must not be the same memory")
             mode = _cabi.PA_QUANT_PER_BLOCK
             st_sb, st_sh = key_scale.stride(0), key_scale.stride(1)
         else:
@@ -147,13 +144,18 @@ def kv_cache_write(
             mode = _cabi.PA_QUANT_PER_TOKEN
             st_sb, st_sh = key_scale.stride(0), key_scale.stride(1)
     st_kc, st_vc = key_cache.stride(), value_cache.stride()
-    if mode == _cabi.PA_QUANT_PER_BLOCK and (st_kc[0] % 16 or st_kc[1] % 16 or st_vc[0] % 16 or st_vc[1] % 16):
-        st_kc, st_vc = _strides(key_cache), _strides(value_cache)
+    ks_ptr, vs_ptr = 0 if key_scale is None else key_scale.data_ptr(), 0 if value_scale is None else value_scale.data_ptr()
+    if mode == _cabi.PA_QUANT_PER_BLOCK:
+        if not (st_sb and st_sh and st_kc[0] and st_kc[1] and st_vc[0] and st_vc[1]):
+            _check_written(key_scale=key_scale, value_scale=value_scale, key_cache=key_cache, value_cache=value_cache)
+        if ks_ptr == vs_ptr and ks_ptr:
+            raise ValueError("key_scale and value_scale are written and must not be the same memory")
+        if st_kc[0] % 16 or st_kc[1] % 16 or st_vc[0] % 16 or st_vc[1] % 16:
+            st_kc, st_vc = _strides(key_cache), _strides(value_cache)
     a = PaKvWriteArgs.from_buffer_copy(_PACK.pack(
         _PACK.size, 0,
         key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-        0 if key_scale is None else key_scale.data_ptr(), 0 if value_scale is None else value_scale.data_ptr(),
-        t, h, d, bs, _cabi.PA_DTYPE_FP8_E4M3FN if key_cache.dtype == FP8_DTYPE else _cabi.PA_DTYPE_BF16, mode, v_transposed,
+        ks_ptr, vs_ptr, t, h, d, bs, _cabi.PA_DTYPE_FP8_E4M3FN if key_cache.dtype == FP8_DTYPE else _cabi.PA_DTYPE_BF16, mode, v_transposed,
         key.stride(0), key.stride(1), value.stride(0), value.stride(1), st_kc[0], st_kc[1], st_vc[0], st_vc[1], st_sb, st_sh))
     lib = _cabi.load_library()
     if mode != _cabi.PA_QUANT_PER_BLOCK:
