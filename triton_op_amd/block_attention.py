@@ -203,7 +203,8 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 class BlockAttentionPlan:
     """A validated call: the filled C struct plus the tensors it points to (kept alive).  `run()` enqueues it on a
     stream; it allocates nothing and can be replayed, and captured.  Plans that may overlap on the GPU need a
-    workspace each (a plan made without one has its own)."""
+    workspace each (a plan made without one has its own).  Keep the plan until its work has run: a workspace of its own
+    goes back to the allocator with it."""
 
     def __init__(self, args: PaBlockArgs, keep, output):
         self.args, self._keep, self.output = args, keep, output
@@ -284,7 +285,8 @@ def plan_block_attention(
         if lse.dtype is not torch.float32 or lse.shape != query.shape[:2] or (lse.stride(1) != 1 and lse.shape[1] > 1):
             raise ValueError(f"lse must be float32 {tuple(query.shape[:2])}, dense over the rows")
         st_lse = lse.stride(0)
-    _check_written(output=output, lse=lse)
+    if not (st_os and st_oh and (st_lse or lse is None)):
+        _check_written(output=output, lse=lse)
     if not output.is_cuda:
         raise ValueError("paged_block_attention runs on the GPU only (there is no CPU path); got a CPU tensor")
     if num_seqs:
@@ -359,7 +361,8 @@ def key_block_bounds(
     st_bb, st_bh = _check_bounds(bounds)
     if bounds.shape != (blocks, heads, 2, head_size):
         raise ValueError(f"bounds shape {tuple(bounds.shape)} is not [{blocks}, {heads}, 2, {head_size}]")
-    _check_written(bounds=bounds)
+    if not (st_bb and st_bh):
+        _check_written(bounds=bounds)
     new, longest = 0 if new_tokens is None else int(new_tokens), max(0, min(int(max_sequence_length), width * bs))
     if new_tokens is not None and new < 1:
         raise ValueError(f"new_tokens must be positive, got {new_tokens}")
@@ -398,7 +401,9 @@ def select_blocks(
     the largest over the head's query rows of sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d), the most that q . k can be for a
     key within the bounds; scores are ranked by their value in 64 bits, ties go to the lower block.  The first
     `first_blocks` and last `recent_blocks` blocks are always taken; `recent_blocks` defaults to, and is at least, the number of
-    blocks the new tokens can lie in."""
+    blocks the new tokens can lie in.  A list is decided in 32 bits with a bound of their error, and many times slower where
+    that does not decide it: more than 65536 blocks, a bound that is no finite number, a table entry outside the cache, a
+    sequence without a query row, or one block of far larger keys than the others' (take the first with `first_blocks`)."""
     dev, index = query.device, query.get_device()
     _check_devices(index, dev, dict(
         bounds=bounds, sequence_lengths=sequence_lengths, block_tables=block_tables, query_lens=query_lens, selected_blocks=selected_blocks,
@@ -422,7 +427,8 @@ def select_blocks(
         raise ValueError(f"num_selected == {num_selected} does not hold first_blocks + recent_blocks == {first_blocks} + {recent}")
     if k * block_size > 1 << 30:
         raise ValueError(f"num_selected == {num_selected} blocks of {block_size} tokens are too many")
-    _check_written(selected_blocks=selected_blocks, selected_counts=selected_counts)
+    if selected_blocks is not None or selected_counts is not None:
+        _check_written(selected_blocks=selected_blocks, selected_counts=selected_counts)
     if not query.is_cuda:
         raise ValueError("select_blocks runs on the GPU only (there is no CPU path); got a CPU tensor")
     if selected_blocks is None:
