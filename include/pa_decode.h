@@ -382,6 +382,7 @@ uint32_t pa_block_args_size(void);
  * merged by a second kernel.  P V is accumulated from probabilities carried as two bf16 terms, so the output's one
  * rounding is the last.  Value rows of all tokens below the context length must be finite: a NaN among a sequence's
  * new tokens reaches all of the sequence's query rows, as 0 * NaN does.  Cache bytes beyond the context are ignored.
+ * Sums are held in f32 with probabilities of up to 2^9: values of more than 2^100 or so may overflow.
  */
 int pa_block_attention(const PaBlockArgs* args, void* hip_stream);
 int64_t pa_block_attention_workspace_bytes(const PaBlockArgs* args);
@@ -398,10 +399,13 @@ int pa_block_bounds(const PaBlockArgs* args, void* hip_stream);
  * For every (sequence, kv head) the num_selected blocks with the largest score, as ascending logical block numbers,
  * -1 behind the last; selected_counts[b, h] of them.  With lo, hi the bounds of a block,
  *     score = max over the sequence's query rows of the head of   sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d),
- * an upper bound of q . k over the block's tokens.  Scores are ranked by their value in 64 bits, equal ones by the lower
- * block number; a row whose sum is not a number is passed over, a block with no other row ranks last.  The first
- * first_blocks and the last recent_blocks blocks of a sequence are always selected (their sum is at most num_selected).
- * The workspace takes pa_select_blocks_workspace_bytes.
+ * the most that q . k can be for a key within the bounds.  (pa_block_bounds rounds to the nearest bf16, so a key may lie outside
+ * its block's bounds by half a bf16 step, 2^-8 of it, and its q . k that much above the score; codes times a power of two
+ * are exact in bf16.)  Scores are ranked by their value in 64 bits, equal ones by the lower block number; a row whose sum
+ * is not a number is passed over, a block with no other row ranks last.  The first first_blocks and the last recent_blocks
+ * blocks of a sequence are always selected (their sum is at most num_selected).  The workspace takes
+ * pa_select_blocks_workspace_bytes.  Lists of more than 65536 blocks, lists with a bound that is no finite number, a bad table
+ * entry or many near-equal scores (one block of far larger keys makes them so) are right and many times slower.
  */
 int pa_select_blocks(const PaBlockArgs* args, void* hip_stream);
 int64_t pa_select_blocks_workspace_bytes(const PaBlockArgs* args);

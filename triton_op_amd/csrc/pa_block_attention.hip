@@ -20,10 +20,12 @@
 // (the rest): one load each per step and lane.
 //
 // Bound by the read of the cache up to 16 query rows per kv head: 64 sequences x 8 heads x 4096 tokens (537 MB) 89 us = 6.0
-// TB/s, 4 x 8 x 131072 tokens 180 us = 6.0 TB/s (a 4 GiB copy reaches 4.8).  A wave has a whole step of K and V in flight, two
-// waves per SIMD.  Three and more tiles (33 .. 64 rows) are bound by the vector ALU, some 350 instructions per tile and
-// step around 48 MFMAs (32 ragged sequences of up to 8191 tokens, 64 rows: 111 us); two tiles per workgroup beat one (144 us
-// with the merge against 125) and four (168: the registers spill).
+// TB/s, 4 x 8 x 131072 tokens 180 us = 6.0 TB/s (a 4 GiB copy reaches 4.8); the first of these with a bf16 cache 5.9 TB/s, with
+// head size 64 5.7 and 256 6.2, in blocks of 64 and 1024 tokens 5.5 and 5.2, with per-token scales 4.5 (head size 256: 3.7, the
+// registers spill).  A wave has a whole step of K and V in flight, two waves per SIMD.  17 .. 32 rows 104 us.  Three and more
+// tiles (33 .. 64 rows) are bound by the vector ALU, some 350 instructions per tile and step around 48 MFMAs (32 ragged sequences of
+// up to 8191 tokens, 64 rows: 111 us); two tiles per workgroup beat one (144 us with the merge against 125) and four (168: the
+// registers spill).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -56,8 +58,9 @@ __device__ __forceinline__ int virtual_tokens(const PaBlockArgs& a, int b, int h
   return ctx > 0 ? n * a.block_size : 0;
 }
 
-// STEP: tokens a wave takes at a time, 64 or 32 (half the registers in flight: head size 256, 16-bit caches, four tiles).  A lane
-// group holds the STEP / 4 consecutive tokens kg * STEP / 4 .. of it, the whole or the half of a 16-token piece.
+// STEP: tokens a wave takes at a time, 64 or 32 (half the registers in flight: head size 256, 16-bit caches, and two tiles with
+// per-token scales at head size 128).  A lane group holds the STEP / 4 consecutive tokens kg * STEP / 4 .. of it, the whole or
+// the half of a 16-token piece.
 // Q_LDS: the query operands wait in LDS (the same for the four waves) and not in registers.
 // OCC: waves per SIMD that the registers are cut for.
 template <int D, bool FP8, int SCALE, int NT, int STEP, int OCC, bool Q_LDS, bool STREAM>

@@ -406,7 +406,9 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 }
 
 // The key of one block's score in 64 bits, by one wave: 8 rows at a time, 8 lanes to a row, 8 head dims of D to a lane and
-// turn.  Products of bf16 numbers are exact in 64 bits, and so are their sums unless the terms are 2^37 apart.
+// turn.  Products of bf16 numbers have 16 significant bits and D of them grow by log2(D) more, so a sum is exact while its terms
+// are no more than 53 - 16 - log2(D) binary orders apart (29 at D = 256).  Beyond that it is a 64-bit sum in this one order: the
+// same for equal bounds, whichever wave forms it.
 __device__ __forceinline__ unsigned long long exact_key(const PaBlockArgs& a, int b, int h, int page, int rows_valid, int lane) {
   double best = -INFINITY;
   if ((unsigned)page < (unsigned)a.num_blocks) {
@@ -444,10 +446,20 @@ __device__ __forceinline__ unsigned long long exact_key(const PaBlockArgs& a, in
 // One workgroup per (sequence, kv head).  The blocks are counted into kBins equal intervals of s; the one in which the count
 // from above reaches `want` holds the threshold, up to the errors e.  Blocks that are above it by more than the
 // errors are taken, blocks below it by more are not, and the few between (the candidates) are ranked by their scores in
-// 64 bits.  With a score that 32 bits do not bound, or more candidates than the list holds (many equal blocks), every score is
-// formed in 64 bits and the threshold is found by eight passes over the keys' bytes.
-// Bound by latency, not by bytes (8 per block, from L2): 5 us for 128 blocks, 8 us for 512 lists of 256, 15 us for 32 of 8192
-// (eight byte passes over 64-bit keys: 68, 88 and 108 us).
+// 64 bits.  Bound by latency, not by bytes (8 per block, from L2): 5 us for 128 blocks, 8 us for 512 lists of 256, 15 us for 32
+// of 8192 (eight byte passes over 64-bit keys: 68, 88 and 108 us).
+//
+// The workgroup forms EVERY score of its list in 64 bits, one block per wave at a time, and finds the threshold by eight passes
+// over the keys' bytes, when
+//   * a list has more than 32 kFlagWords = 65536 blocks;
+//   * one of its scores is not bounded by 32 bits (e = infinity): a bound that is infinite or NaN, a table entry outside the
+//     cache, or a sequence without a query row;
+//   * more than kCandidates blocks are left between: many equal blocks, or one whose keys are far larger than the others', which
+//     widens all bins and the list's largest error E.
+// The list is the same, the time is not: 32 lists of 8192 blocks, scores and selection together, 44 us for 256 of them, 74 with
+// one block of 30 times the keys, 2.0 ms with one of 100 times (1024 of them: 48 us, 146 us, 2.0 ms), 2.0 ms with one bad entry;
+// 8 lists of 65536 blocks 116 us, of 65537 16 ms.  The blocks that are always taken are not among the scores: first_blocks = 1
+// spares a list its first block's large keys.
 constexpr int kSelectThreads = 512;
 constexpr int kAhead = 4;
 constexpr int kSelectWaves = kSelectThreads / 64;

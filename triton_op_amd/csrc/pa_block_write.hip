@@ -12,7 +12,10 @@
 // change, 16 bytes of a row per lane.  K leaves as 8-byte halves of (chunk, token) cells, V is turned in LDS so that a
 // head dim's 16 tokens are one 16-byte store, new codes among the old ones.  Every byte is written at most once.
 // Bound by the chain of latencies slot -> slot mapping -> rows -> store: 64 tokens x 8 heads 8 us, 8192 tokens (50 MB) 22 us = 2.3
-// TB/s; the read of the slot mapping grows with its square (65536 tokens: 255 us).
+// TB/s in blocks of 16; the read of the slot mapping grows with its square (65536 tokens: 260 us).
+// Larger blocks have fewer owners, and a wave goes through its block's segments one after the other, twice: 8192 tokens take 46 us in
+// blocks of 64 and 0.52 ms in blocks of 1024 (8 workgroups at work).  A scale that grows rewrites the whole block, also slots
+// that hold nothing yet: a step of 64 tokens whose scales all grow takes 8, 20 and 250 us in blocks of 16, 64 and 1024.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -330,6 +333,7 @@ extern "C" int pa_kv_cache_write_block_scaled(const PaKvWriteArgs* a, int64_t nu
   if ((caches & 15) || a->stride_kc_b % 16 || a->stride_kc_h % 16 || a->stride_vc_b % 16 || a->stride_vc_h % 16) return PA_ERR_BAD_SHAPE;
   const uintptr_t rows = reinterpret_cast<uintptr_t>(a->key) | reinterpret_cast<uintptr_t>(a->value);
   const bool aligned = (rows & 15) == 0 && a->stride_k_t % 8 == 0 && a->stride_k_h % 8 == 0 && a->stride_v_t % 8 == 0 && a->stride_v_h % 8 == 0;
+  // (Both cuts are for blocks of 16 tokens; larger blocks have the same.)
   // A few tokens (decode): one workgroup per (token, four kv heads).  Many (prompts): most tokens own no block, so a
   // workgroup looks at four of them, and walks all kv heads so that the slot mapping is read once per block (8192 tokens, 8
   // heads: 28 us with windows of 16, where one workgroup in a prompt has two blocks, 23 with 4).
